@@ -19,8 +19,10 @@ HEADERS = [os.path.join(CSRC, "sig3d_common.h"), os.path.join(CSRC, "shared_mlp_
            os.path.join(HERE, "..", "include", "sig3d_hip.h"), os.path.join(HERE, "..", "include", "sig3d_debug.h")]
 # -ffp-contract=off: distances are spelled with _rn intrinsics already; this keeps every other
 # f32 expression in the point ops unfused too (parity contract, see oracle/pointnet2_oracle.c).
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on MI355X); the host pass
+# warns that it does not know the feature.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
-         "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function"]
+         "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
