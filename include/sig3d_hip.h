@@ -851,6 +851,85 @@ int sig3d_bn_relu_bwd_compact(int b, int c, long e, int p, const float *dA, cons
                               const int *n_act, const float *mult, const int *centre_of, const int *seg_off,
                               void *stream);
 
+/* ---- language side: attention with a relative position bias, key / value cache, decoding over shared prefixes ----------
+ * The operators of the language head behind the point branch (blip2_t5.py:102-183; its attention is modeling_t5.py's): the
+ * reference runs them as torch operations over a materialised (b, h, nq, nk) score and bias tensor.
+ * dtype: 0 float32, 1 bfloat16, 2 float16.  Every tensor is dense in its innermost dimension; the strides given here are in
+ * elements; addresses and strides (in bytes) are multiples of 16.  d: 64, 96 or 128; h a multiple of hkv, head i reads key
+ * head i / (h / hkv).  No call records a memset node; results do not depend on the order in which workgroups run.  The _work_floats functions return -1 for arguments
+ * that the calls refuse. */
+#define SIG3D_REL_MAX_BUCKETS 128   /* of one direction */
+#define SIG3D_REL_MAX_REACH 1024    /* largest border */
+
+/* border[i] (non-decreasing, border[0] = 0) is the smallest distance of bucket i of one direction: distance a is in the
+ * last bucket with border[i] <= a.  both != 0: keys ahead of the query have buckets n .. 2n-1 of their own, else they share
+ * bucket 0.  n = 0: no bias. */
+typedef struct {
+  int n, both;
+  int border[SIG3D_REL_MAX_BUCKETS];
+} sig3d_rel_buckets;
+
+/* q (b, nq, h, d), k / v (b, nk, hkv, d); query i stands at position p = i + query_offset and sees key j when
+ *   j < key_lengths[b]  and  (!causal or j <= p or j < prefix_lengths[b])  and  key_ranges[b][i][0] <= j < key_ranges[b][i][1]
+ * (arrays that are NULL say nothing; prefix_lengths only matters with causal).
+ *   s_ij = scale q_i.k_j + table[bucket(j - p)][head],   out_i = sum_j softmax_j(s_i) v_j,   0 where a query sees no key.
+ * Key rows outside the interval that the queries of a workgroup see are taken as zero: padding may hold anything. */
+typedef struct {
+  const void *q, *k, *v, *table;              /* table (table_rows, h) dense, of dtype */
+  const int *key_lengths, *prefix_lengths, *key_ranges;
+  void *out;                                  /* (b, nq, h, d) dense, of dtype */
+  float *out32, *lse;                         /* for the backward pass (both or neither): out unrounded; (b, h, nq) log2 of the
+                                                 sum of exponentials, +inf where a query sees no key */
+  const void *grad;                           /* backward: d out */
+  void *dq, *dk, *dv, *dtable;                /* backward: dense, of dtype; dtable NULL without a bias */
+  float *work;                                /* backward: sig3d_rel_attention_bwd_work_floats() floats */
+  long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, grad_b, grad_n, grad_h;
+  int dtype, b, nq, nk, h, hkv, d, causal, query_offset, table_rows;
+  float scale;
+  sig3d_rel_buckets buckets;
+} sig3d_rel_attention_args;
+int sig3d_rel_attention_fwd(const sig3d_rel_attention_args *args, void *stream);
+int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *args, void *stream);
+long sig3d_rel_attention_bwd_work_floats(const sig3d_rel_attention_args *args);
+
+/* A cache of b sequences: k_cache / v_cache (b, hkv, capacity, d), of dtype, or e4m3 (OCP, 1 byte) with one f32 scale per
+ * row, k_scale / v_scale (b, hkv, capacity): the smallest power of two with max |row| <= 448 scale, values rounded to
+ * nearest even; infinite values are held as +-448 scale and do not count in the maximum, NaN stays NaN. */
+typedef struct {
+  const void *k, *v;                          /* (b, t, hkv, d): new tokens */
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;                   /* NULL: the cache is of dtype */
+  const int *start, *counts;                  /* (b) or NULL: token i < counts[b] (default t) goes to row start[b] + i (default
+                                                 lengths[b] + i); rows outside [0, capacity) are dropped */
+  int *lengths;                               /* (b): set to start + counts, at most capacity */
+  long k_b, k_n, k_h, v_b, v_n, v_h;
+  int dtype, b, t, capacity, hkv, d;
+} sig3d_cache_append_args;
+int sig3d_cache_append(const sig3d_cache_append_args *args, void *stream);
+/* k_out / v_out (b, n, hkv, d) dense, of dtype: the values that the first n rows hold, zeros from lengths[b] on */
+int sig3d_cache_read(int dtype, int b, int n, int capacity, int hkv, int d, const void *k_cache, const void *v_cache,
+                     const float *k_scale, const float *v_scale, const int *lengths, void *k_out, void *v_out, void *stream);
+
+/* Attention of new tokens over the cache they have been appended to.  Sequence i sees the rows of shared sequence
+ * i / (b / groups), [0, shared_lengths[.]), then its own: with n = counts[i] (default t) new tokens, query j < n is the token
+ * in own row lengths[i] - n + j, and sees the own rows up to it.  Its position, and that of every key, counts the shared rows
+ * first.  out (b, t, h, d) dense: 0 for j >= n, for rows before the first, and where nothing is seen.
+ * scores and bias as above.  groups = 0: nothing shared. */
+typedef struct {
+  const void *q, *table;
+  const void *k_cache, *v_cache, *shared_k, *shared_v;
+  const float *k_scale, *v_scale, *shared_k_scale, *shared_v_scale;
+  const int *lengths, *shared_lengths, *counts;
+  void *out;
+  float *work;                                /* sig3d_decode_attention_work_floats() floats; may be NULL when that is 0 */
+  long q_b, q_n, q_h;
+  int dtype, b, t, h, hkv, d, capacity, groups, shared_capacity, table_rows;
+  float scale;
+  sig3d_rel_buckets buckets;
+} sig3d_decode_attention_args;
+int sig3d_decode_attention(const sig3d_decode_attention_args *args, void *stream);
+long sig3d_decode_attention_work_floats(const sig3d_decode_attention_args *args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -251,6 +251,47 @@ def planes_split(src, planes, rows=None, chunk_rows=None):
     return planes
 
 
+REL_MAX_BUCKETS, REL_MAX_REACH = 128, 1024
+
+
+class RelBuckets(ctypes.Structure):
+    """sig3d_rel_buckets of include/sig3d_hip.h."""
+    _fields_ = [("n", _I), ("both", _I), ("border", _I * REL_MAX_BUCKETS)]
+
+
+class RelAttentionArgs(ctypes.Structure):
+    """sig3d_rel_attention_args of include/sig3d_hip.h (field order and types must match)."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "table", "key_lengths", "prefix_lengths", "key_ranges", "out", "out32", "lse",
+                                   "grad", "dq", "dk", "dv", "dtable", "work")]
+                + [(n, ctypes.c_long) for n in ("q_b", "q_n", "q_h", "k_b", "k_n", "k_h", "v_b", "v_n", "v_h", "grad_b", "grad_n",
+                                                "grad_h")]
+                + [(n, _I) for n in ("dtype", "b", "nq", "nk", "h", "hkv", "d", "causal", "query_offset", "table_rows")]
+                + [("scale", _F), ("buckets", RelBuckets)])
+
+
+class CacheAppendArgs(ctypes.Structure):
+    """sig3d_cache_append_args of include/sig3d_hip.h."""
+    _fields_ = ([(n, _P) for n in ("k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "start", "counts", "lengths")]
+                + [(n, ctypes.c_long) for n in ("k_b", "k_n", "k_h", "v_b", "v_n", "v_h")]
+                + [(n, _I) for n in ("dtype", "b", "t", "capacity", "hkv", "d")])
+
+
+class DecodeAttentionArgs(ctypes.Structure):
+    """sig3d_decode_attention_args of include/sig3d_hip.h."""
+    _fields_ = ([(n, _P) for n in ("q", "table", "k_cache", "v_cache", "shared_k", "shared_v", "k_scale", "v_scale",
+                                   "shared_k_scale", "shared_v_scale", "lengths", "shared_lengths", "counts", "out", "work")]
+                + [(n, ctypes.c_long) for n in ("q_b", "q_n", "q_h")]
+                + [(n, _I) for n in ("dtype", "b", "t", "h", "hkv", "d", "capacity", "groups", "shared_capacity", "table_rows")]
+                + [("scale", _F), ("buckets", RelBuckets)])
+
+
+SIGNATURES["sig3d_rel_attention_fwd"] = [ctypes.POINTER(RelAttentionArgs), _P]
+SIGNATURES["sig3d_rel_attention_bwd"] = [ctypes.POINTER(RelAttentionArgs), _P]
+SIGNATURES["sig3d_cache_append"] = [ctypes.POINTER(CacheAppendArgs), _P]
+SIGNATURES["sig3d_cache_read"] = [_I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["sig3d_decode_attention"] = [ctypes.POINTER(DecodeAttentionArgs), _P]
+
+
 class BqLevel(ctypes.Structure):
     """sig3d_bq_level of include/sig3d_hip.h: one ball-query problem of a multi-level launch."""
     _fields_ = [("n", _I), ("m", _I), ("nsample", _I), ("radius", _F), ("xyz", _P), ("new_xyz", _P), ("idx", _P)]
@@ -299,7 +340,8 @@ def bq_levels_workspace_bytes(batch, arr):
 
 INFO_SYMBOLS = ("sig3d_version", "sig3d_last_error", "sig3d_voxelize_workspace_bytes", "sig3d_fps_blocks_workspace_bytes",
                 "sig3d_ball_query_levels_workspace_bytes", "sig3d_pooled_heads_work_floats",
-                "sig3d_mlp_layer_dw_stream_work_floats", "sig3d_gemmp_work_floats")
+                "sig3d_mlp_layer_dw_stream_work_floats", "sig3d_gemmp_work_floats", "sig3d_rel_attention_bwd_work_floats",
+                "sig3d_decode_attention_work_floats")
 
 _lib = None
 
@@ -335,6 +377,10 @@ def load():
     lib.sig3d_pooled_heads_work_floats.restype = ctypes.c_long
     lib.sig3d_mlp_layer_dw_stream_work_floats.argtypes = [_I, _I, _I, ctypes.c_long]
     lib.sig3d_mlp_layer_dw_stream_work_floats.restype = ctypes.c_long
+    lib.sig3d_rel_attention_bwd_work_floats.argtypes = [ctypes.POINTER(RelAttentionArgs)]
+    lib.sig3d_rel_attention_bwd_work_floats.restype = ctypes.c_long
+    lib.sig3d_decode_attention_work_floats.argtypes = [ctypes.POINTER(DecodeAttentionArgs)]
+    lib.sig3d_decode_attention_work_floats.restype = ctypes.c_long
     _lib = lib
     return lib
 

@@ -1,0 +1,483 @@
+// decode_attention.hip -- attention of new tokens over the key / value cache, with prefixes that many sequences share, for gfx950.
+//
+// Sequence i sees [the rows of shared sequence i / (b / groups) | its own rows up to the query].  Decoding is bound by reading
+// keys and values, so each part is read as few times as its users allow: the queries of ALL sequences of a group that share a
+// key head are rows of one product over the shared keys (up to 64 rows a workgroup), and only the own rows are read per
+// sequence.  Both parts are cut along the keys until the chip is full; a piece leaves (max, sum, unnormalised output), and a
+// second kernel joins the pieces of a row in their order.  Small calls -- one piece, nothing worth sharing -- are one launch:
+// a workgroup walks shared and own rows of one sequence and writes the result itself.
+//
+// A wave owns every fourth 32-key tile of its workgroup's piece and NB blocks of 16 query rows; no barrier until the waves join.
+// S^T = K Q^T on 16x16x32: the K fragment is loaded straight from memory (a lane's 16 bytes are a fragment), in the row order
+// that makes two S tiles' registers the P fragment (key 8 g + 4 t + r for tile t, lane group g, register r).  V is staged in
+// wave-private LDS for the transposing read.  The next tile's loads are in flight while one is used.
+// An e4m3 cache is widened to the query's type on the way in -- exact, the scale being a power of two.
+#include "lang_core.h"
+
+#include <limits.h>
+
+#include <algorithm>
+
+namespace {
+using namespace lang;
+
+constexpr int WAVES = 4, KT = 32;
+
+struct Side { const void *k, *v; const float *k_scale, *v_scale; int capacity; };
+struct DecodeParams {
+  const void *q, *table;
+  Side own, shared;
+  const int *lengths, *shared_lengths, *counts;
+  void *out;
+  float *part;               // pieces: D + 2 floats a row and piece (output, max, sum)
+  long q_b, q_n, q_h;
+  int b, t, h, hkv, group, each;       // each: sequences of a shared prefix (0: nothing is shared)
+  int own_splits, shared_splits, own_tiles, shared_tiles, shared_items, bias_heads;
+  int joined;                // own items walk the shared rows too, no shared items
+  int direct;                // one piece a row: the result is written here
+  float scale;
+  Buckets bk;
+};
+
+// One 32-key tile of one side on its way from memory.
+template <typename T, int D, bool Q> struct Flight {
+  static constexpr int KS = D / 32;                         // reduction steps of a score
+  static constexpr int VN = D / 16;                         // 8-element pieces of V a lane carries
+  frag_t<T> k[2][Q ? 1 : KS];
+  uint2 kq[2][Q ? KS : 1];
+  float ks[2];
+  frag_t<T> v[Q ? 1 : VN];
+  uint2 vq[Q ? VN : 1];
+  float vs[Q ? VN : 1];
+
+  __device__ __forceinline__ void load(const Side &s, long row0, int k0, int end, int lane) {
+    const int m = lane & 15, g = lane >> 4, last = end - 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const long row = row0 + min(k0 + 8 * (m >> 2) + 4 * t + (m & 3), last);      // beyond the end: any row, masked later
+      if constexpr (Q) {
+        ks[t] = s.k_scale[row];
+#pragma unroll
+        for (int f = 0; f < KS; ++f)       // lane group g holds D / 4 consecutive values: 16 bytes a load, and Q likewise
+          kq[t][f] = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(s.k) + row * D + g * (D / 4) + 8 * f);
+      } else {
+#pragma unroll
+        for (int f = 0; f < KS; ++f)
+          k[t][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(s.k) + row * D + 32 * f + 8 * g);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int c = lane + 64 * i, r = c / (D / 8), o = c - r * (D / 8);
+      const bool ok = k0 + r < end;
+      const long row = row0 + k0 + r;
+      if constexpr (Q) {
+        vq[i] = make_uint2(0, 0);
+        vs[i] = 1.f;
+        if (ok) {
+          vq[i] = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(s.v) + row * D + 8 * o);
+          vs[i] = s.v_scale[row];
+        }
+      } else {
+        v[i] = frag_t<T>{};
+        if (ok) v[i] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(s.v) + row * D + 8 * o);
+      }
+    }
+  }
+  __device__ __forceinline__ frag_t<T> key(int t, int f) const {
+    if constexpr (Q) return from_e4m3<T>(kq[t][f], ks[t]);
+    else return k[t][f];
+  }
+  __device__ __forceinline__ void put_v(char *tile, int lane) const {
+    typedef Tile<T, D> TL;
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int c = lane + 64 * i, r = c / (D / 8), o = c - r * (D / 8);
+      frag_t<T> x;
+      if constexpr (Q) x = from_e4m3<T>(vq[i], vs[i]);
+      else x = v[i];
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<frag_t<T> *>(tile + TL::at(r, o)) = x;
+      } else {
+        *reinterpret_cast<f32x4 *>(tile + TL::at(r, 2 * o)) = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+        *reinterpret_cast<f32x4 *>(tile + TL::at(r, 2 * o + 1)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+      }
+    }
+  }
+};
+
+// which element of a head fragment f of lane group g starts at (see Flight::load)
+template <int D, bool Q> __device__ __forceinline__ int element(int f, int g) { return Q ? g * (D / 4) + 8 * f : 32 * f + 8 * g; }
+
+__device__ __forceinline__ float max_groups(float x) {      // over the four 16-lane groups
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return max_halves(x);
+}
+__device__ __forceinline__ float sum_groups(float x) {
+  x += __shfl_xor(x, 16);
+  return sum_halves(x);
+}
+
+// What one row of queries is.
+struct RowInfo { int head, j, seq, pos, end; };    // pos: own row of the query (below 0: no query); end = pos + 1 own rows seen
+
+template <typename T, int D, bool Q, int NB>
+__device__ __forceinline__ void walk(const DecodeParams &p, int item, bool shared, char *lds) {
+  typedef Tile<T, D> TL;
+  typedef Flight<T, D, Q> FL;
+  constexpr int KS = FL::KS, TB = KT * TL::ROW, DT = D / 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  char *vt = lds + wave * TB;
+  float *bias = reinterpret_cast<float *>(lds + WAVES * TB);
+  float *stat = bias + p.bias_heads * (p.bk.reach + 1);                    // [2][WAVES][16]
+
+  // item -> (sequence or group, key head, block of rows, piece)
+  const int splits = shared ? p.shared_splits : p.own_splits, tiles = shared ? p.shared_tiles : p.own_tiles;
+  const int piece = item % splits;
+  item /= splits;
+  const int rt = item % tiles;
+  item /= tiles;
+  const int kvh = item % p.hkv, unit = item / p.hkv;                       // unit: sequence, or group
+  const int per = p.group * p.t, rows = shared ? p.each * per : per;
+  const int r0 = rt * 16 * NB;
+
+  RowInfo info[NB];
+  frag_t<T> qf[NB][KS];
+  const int shared_len = p.each ? (shared || p.joined ? min(max(p.shared_lengths[shared ? unit : unit / p.each], 0), p.shared.capacity) : 0) : 0;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int r = r0 + 16 * n + col, in = r % per;
+    info[n].seq = shared ? unit * p.each + r / per : unit;
+    info[n].head = kvh * p.group + in / p.t;
+    info[n].j = in % p.t;
+    info[n].pos = -1;
+    if (r < rows) {
+      const int len = min(max(p.lengths[info[n].seq], 0), p.own.capacity);
+      const int count = p.counts ? min(max(p.counts[info[n].seq], 0), p.t) : p.t;
+      if (info[n].j < count) info[n].pos = max(len - count + info[n].j, -1);
+    }
+    info[n].end = info[n].pos + 1;
+    const bool ok = info[n].pos >= 0;
+#pragma unroll
+    for (int f = 0; f < KS; ++f) {
+      qf[n][f] = frag_t<T>{};
+      if (ok)
+        qf[n][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.q) + info[n].seq * p.q_b +
+                                                       (long)info[n].j * p.q_n + info[n].head * p.q_h + element<D, Q>(f, g));
+    }
+  }
+  const bool biased = p.bk.n > 0;
+  const int head0 = kvh * p.group + (r0 % per) / p.t, reach = p.bk.reach;
+  const T *table = reinterpret_cast<const T *>(p.table);
+  if (biased) {        // log2(e) * bias of the heads of these rows by distance behind the query
+    for (int i = tid; i < p.bias_heads * (reach + 1); i += WAVES * 64) {
+      const int hh = i / (reach + 1), a = i - hh * (reach + 1);
+      const int head = kvh * p.group + (head0 - kvh * p.group + hh) % p.group;
+      bias[i] = (float)table[(long)bucket_of(p.bk, -a) * p.h + head] * LOG2E;
+    }
+    __syncthreads();
+  }
+  const float *mine[NB];
+  float farthest[NB];
+  int longest = 0, lowest = INT_MAX;         // own rows seen by any row here; lowest position of a query
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    int hh = info[n].head - head0;
+    if (hh < 0) hh += p.group;
+    mine[n] = bias + min(hh, max(p.bias_heads - 1, 0)) * (reach + 1);
+    farthest[n] = biased ? mine[n][reach] : 0.f;
+    longest = max(longest, info[n].end);
+    if (info[n].pos >= 0) lowest = min(lowest, info[n].pos);
+  }
+  longest = wave_max_i32(longest);
+  lowest = wave_min_i32(lowest);
+
+  f32x4 o[NB][DT] = {};
+  float m[NB], l[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) { m[n] = -INFINITY; l[n] = 0.f; }
+  const float scale2 = p.scale * LOG2E;
+
+  // the piece: tiles of the shared rows, then of the own rows
+  const int own_len = shared ? 0 : longest, far_len = longest > 0 ? shared_len : 0;
+  const int far_tiles = (far_len + KT - 1) / KT, all_tiles = far_tiles + (own_len + KT - 1) / KT;
+  const int share = (all_tiles + splits - 1) / splits, from = piece * share, to = min(from + share, all_tiles);
+  const long far_row = ((long)(shared ? unit : (p.each ? unit / p.each : 0)) * p.hkv + kvh) * p.shared.capacity;
+  const long own_row = ((long)unit * p.hkv + kvh) * p.own.capacity;
+  FL fl;
+  auto fetch = [&](int tile) {
+    const bool far = tile < far_tiles;
+    fl.load(far ? p.shared : p.own, far ? far_row : own_row, (far ? tile : tile - far_tiles) * KT, far ? far_len : own_len, lane);
+  };
+  if (from + wave < to) fetch(from + wave);
+  for (int tile = from + wave; tile < to; tile += WAVES) {
+    const bool far = tile < far_tiles;
+    const int k0 = (far ? tile : tile - far_tiles) * KT, end = far ? far_len : own_len;
+    // distance of a query at own row pos from key 0 of the tile: shared rows stand before the own ones
+    const int ahead = far ? shared_len - k0 : -k0;
+    f32x4 s[NB][2] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int f = 0; f < KS; ++f) {
+        const frag_t<T> kf = fl.key(t, f);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n][t] = mma16(kf, qf[n][f], s[n][t]);
+      }
+    fl.put_v(vt, lane);
+    if (tile + WAVES < to) fetch(tile + WAVES);
+    const bool near = biased && lowest + ahead - (KT - 1) < reach;
+    const bool cut = k0 + KT > end || (!far && k0 + KT > lowest + 1);
+    frag_t<T> pf[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_fmaf(s[n][j >> 2][j & 3], scale2, near ? 0.f : farthest[n]);
+      if (near) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += mine[n][min(max(info[n].pos + ahead - 8 * g - j, 0), reach)];
+      }
+      if (cut) {
+        const int seen = far ? end : min(end, info[n].end);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (k0 + 8 * g + j >= seen) x[j] = -INFINITY;
+      }
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+      top = max_groups(top);
+      if (__any(top > m[n])) {
+        const float now = fmaxf(m[n], top);
+        const float keep = now == -INFINITY ? 1.f : exp2_(m[n] - now);
+        m[n] = now;
+        l[n] *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[n][d][r] *= keep;
+      }
+      const float base = m[n] == -INFINITY ? 0.f : m[n];
+      f32x8 e;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = exp2_(x[j] - base);
+        l[n] += e[j];
+      }
+      pf[n] = to_frag<T>(e);
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const frag_t<T> vf = TL::col_frag(vt, 8 * g, 16 * d, lane);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) o[n][d] = mma16(vf, pf[n], o[n][d]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // join the four waves, one block of 16 rows at a time: a wave leaves its output, scaled to the common maximum, in LDS
+  float *mine_o = reinterpret_cast<float *>(lds);                           // [WAVES][16][D]; the V tiles are done with
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const bool live = info[n].pos >= 0;                                     // what is no query has seen the shared rows for nothing
+    const float sum = live ? sum_groups(l[n]) : 0.f;
+    if (!live) m[n] = -INFINITY;
+    __syncthreads();
+    if (g == 0) {
+      stat[wave * 16 + col] = m[n];
+      stat[(WAVES + wave) * 16 + col] = sum;
+    }
+    __syncthreads();
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stat[w * 16 + col]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) total += stat[(WAVES + w) * 16 + col] * exp2_(stat[w * 16 + col] - base);
+    const float keep = exp2_(m[n] - base);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      f32x4 x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = live ? o[n][d][r] * keep : 0.f;
+      // 16-byte slots of a row rotate with the row: the 16 rows of a store instruction spread over the banks
+      *reinterpret_cast<f32x4 *>(mine_o + (wave * 16 + col) * D + ((4 * d + g + col) % (D / 4)) * 4) = x;
+    }
+    __syncthreads();
+    constexpr int PER = D / 4;                                              // 16-byte slots of a row
+    if (g == 0 && wave == 0) { stat[col] = top; stat[WAVES * 16 + col] = total; }
+    __syncthreads();
+    for (int i = tid; i < 16 * PER; i += WAVES * 64) {
+      const int c = i / PER, e = i - c * PER, r = r0 + 16 * n + c;
+      if (r >= rows) continue;
+      f32x4 x = {};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(mine_o + (w * 16 + c) * D + ((e + c) % PER) * 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] += y[q];
+      }
+      const float rt_max = stat[c], rt_sum = stat[WAVES * 16 + c];
+      if (p.direct) {
+        const int in = r % per, seq = shared ? unit * p.each + r / per : unit;
+        const float inv = rt_sum > 0.f || rt_sum != rt_sum ? 1.f / rt_sum : 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] *= inv;
+        const long at = (((long)seq * p.t + in % p.t) * p.h + kvh * p.group + in / p.t) * D + 4 * e;
+        *reinterpret_cast<vec4_t<T> *>(reinterpret_cast<T *>(p.out) + at) = to_vec4<T>(x);
+      } else {
+        // pieces of a row lie side by side: [shared rows' | own rows'] [row][piece][D + 2]
+        const long base_row = shared ? 0 : (long)p.shared_splits * p.b * p.hkv * per;
+        float *to_ = p.part + (base_row + (((long)unit * p.hkv + kvh) * rows + r) * splits + piece) * (D + 4);
+        *reinterpret_cast<f32x4 *>(to_ + 4 * e) = x;
+        if (e == 0) { to_[D] = rt_max; to_[D + 1] = rt_sum; }
+      }
+    }
+  }
+}
+
+template <typename T, int D, bool Q, int NB>
+__global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p) {
+  extern __shared__ __align__(16) char lds[];
+  if ((int)blockIdx.x < p.shared_items) walk<T, D, Q, NB>(p, blockIdx.x, true, lds);
+  else walk<T, D, Q, 1>(p, blockIdx.x - p.shared_items, false, lds);
+}
+
+// Joins the pieces of a row, shared ones first: D / 4 lanes a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
+  constexpr int PER = D / 4, ROWS = 256 / PER;
+  const int per = p.group * p.t, e = threadIdx.x % PER;
+  const long row = (long)blockIdx.x * ROWS + threadIdx.x / PER;              // (sequence, key head, head of the group, token)
+  if (threadIdx.x / PER >= ROWS || row >= (long)p.b * p.hkv * per) return;
+  const int in = (int)(row % per);
+  const int kvh = (int)(row / per % p.hkv), seq = (int)(row / per / p.hkv);
+  const float *own = p.part + ((long)p.shared_splits * p.b * p.hkv * per + row * p.own_splits) * (D + 4);
+  const float *far = nullptr;
+  if (p.shared_splits)
+    far = p.part + ((((long)(seq / p.each) * p.hkv + kvh) * p.each + seq % p.each) * per + in) * p.shared_splits * (D + 4);
+  float top = -INFINITY;
+  for (int s = 0; s < p.shared_splits; ++s) top = fmaxf(top, far[s * (D + 4) + D]);
+  for (int s = 0; s < p.own_splits; ++s) top = fmaxf(top, own[s * (D + 4) + D]);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 x = {};
+  float sum = 0.f;
+  auto add = [&](const float *piece) {
+    const float keep = exp2_(piece[D] - base);
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(piece + 4 * e);
+    sum += piece[D + 1] * keep;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(y[q], keep, x[q]);
+  };
+  for (int s = 0; s < p.shared_splits; ++s) add(far + s * (D + 4));
+  for (int s = 0; s < p.own_splits; ++s) add(own + s * (D + 4));
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) x[q] *= inv;
+  const long at = (((long)seq * p.t + in % p.t) * p.h + kvh * p.group + in / p.t) * D + 4 * e;
+  *reinterpret_cast<vec4_t<T> *>(reinterpret_cast<T *>(p.out) + at) = to_vec4<T>(x);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+struct Plan { int nb, own_splits, shared_splits, own_tiles, shared_tiles, shared_items, own_items, bias_heads, joined, direct; size_t lds; };
+
+int check(const char *where, const sig3d_decode_attention_args *a) {
+  LANG_NEED(where, a != nullptr, "no arguments");
+  LANG_NEED(where, a->dtype >= 0 && a->dtype <= 2, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+  LANG_NEED(where, a->d == 64 || a->d == 96 || a->d == 128, "head size must be 64, 96 or 128");
+  LANG_NEED(where, a->b >= 1 && a->t >= 1 && a->h >= 1 && a->hkv >= 1 && a->capacity >= 1, "sizes must be positive");
+  LANG_NEED(where, a->h % a->hkv == 0, "heads must be a multiple of key heads");
+  LANG_NEED(where, a->capacity <= (1 << 29) && a->shared_capacity <= (1 << 29), "at most 2^29 rows");
+  LANG_NEED(where, a->groups >= 0 && (a->groups == 0 || a->b % a->groups == 0), "groups must divide the batch");
+  LANG_NEED(where, a->groups == 0 || a->shared_capacity >= 1, "shared sequences without rows");
+  LANG_NEED(where, (long)a->b * a->t * a->h < (1l << 24), "too many query rows");
+  return check_buckets(where, a->buckets, a->table, a->table_rows);
+}
+
+Plan plan(const sig3d_decode_attention_args *a) {
+  Plan s = {};
+  const int group = a->h / a->hkv, per = group * a->t, each = a->groups ? a->b / a->groups : 0;
+  const int reach = a->buckets.n ? device_buckets(a->buckets).reach : 0;
+  s.own_tiles = sig3d_ceil_div(per, 16);
+  const long base = (long)a->b * a->hkv * s.own_tiles;
+  // Walking the shared rows once a sequence costs nothing where no other sequence shares them, and one launch instead of two
+  // where they are short.
+  s.joined = each > 0 && (each == 1 || a->shared_capacity <= 256);
+  s.nb = 1;
+  const int piece = 8 * KT;             // two tiles a wave: a piece below that is all start and join
+  const int own_rows = a->capacity + (s.joined ? a->shared_capacity : 0);
+  s.own_splits = (int)std::min<long>(std::max<long>(1, 1024 / base), sig3d_ceil_div(own_rows, piece));
+  if (each > 0 && !s.joined) {
+    const long rows = (long)each * per;
+    s.nb = rows > 16 ? 4 : 1;
+    s.shared_tiles = sig3d_ceil_div(rows, 16 * s.nb);
+    const long far = (long)a->groups * a->hkv * s.shared_tiles;
+    s.shared_splits = (int)std::min<long>(std::max<long>(1, 1024 / far), sig3d_ceil_div(a->shared_capacity, piece));
+    s.shared_items = (int)(far * s.shared_splits);
+  }
+  s.own_items = (int)(base * s.own_splits);
+  s.direct = s.own_splits == 1 && !s.shared_splits;
+  const int e = a->dtype == 0 ? 4 : 2, row = (a->d * e / 16 + 7) / 8 * 8 * 16;
+  s.bias_heads = a->buckets.n ? std::min(group, (16 * s.nb + a->t - 2) / a->t + 1) : 0;
+  s.lds = std::max<size_t>(WAVES * KT * row, WAVES * 16 * a->d * 4) + (size_t)s.bias_heads * (reach + 1) * 4 + 2 * WAVES * 16 * 4;
+  return s;
+}
+
+template <typename T, int D, bool Q, int NB> int launch(const DecodeParams &p, const Plan &s, hipStream_t stream) {
+  static sig3d_once_per_device once;
+  if (int e = allow_lds(decode_kernel<T, D, Q, NB>, once)) return e;
+  decode_kernel<T, D, Q, NB><<<s.shared_items + s.own_items, WAVES * 64, s.lds, stream>>>(p);
+  SIG3D_LAUNCH_CHECK("decode_kernel");
+  if (!p.direct) {
+    const long rows = (long)p.b * p.hkv * p.group * p.t;
+    decode_join_kernel<T, D><<<sig3d_ceil_div(rows, 256 / (D / 4)), 256, 0, stream>>>(p);
+    SIG3D_LAUNCH_CHECK("decode_join_kernel");
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" long sig3d_decode_attention_work_floats(const sig3d_decode_attention_args *a) {
+  if (check("sig3d_decode_attention_work_floats", a)) return -1;
+  const Plan s = plan(a);
+  return s.direct ? 0 : (long)a->b * a->t * a->h * (s.own_splits + s.shared_splits) * (a->d + 4);
+}
+
+extern "C" int sig3d_decode_attention(const sig3d_decode_attention_args *a, void *stream) {
+  if (int e = check("sig3d_decode_attention", a)) return e;
+  const Plan s = plan(a);
+  SIG3D_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->lengths && (s.direct || a->work), "missing array");
+  SIG3D_REQUIRE(a->groups == 0 || (a->shared_k && a->shared_v && a->shared_lengths), "missing shared array");
+  const bool quantized = a->k_scale != nullptr;
+  SIG3D_REQUIRE((a->v_scale != nullptr) == quantized && (a->groups == 0 || ((a->shared_k_scale != nullptr) == quantized &&
+                (a->shared_v_scale != nullptr) == quantized)), "own and shared rows must be held alike");
+  SIG3D_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->k_cache) && aligned16(a->v_cache) && aligned16(a->shared_k) &&
+                aligned16(a->shared_v) && aligned16(a->work), "addresses must be 16-byte aligned");
+  const int e = a->dtype == 0 ? 4 : 2;
+  SIG3D_REQUIRE(a->q_b >= 0 && a->q_n >= 0 && a->q_h >= 0 && a->q_b * e % 16 == 0 && a->q_n * e % 16 == 0 && a->q_h * e % 16 == 0,
+                "strides must be non-negative multiples of 16 bytes");
+  SIG3D_REQUIRE((long)a->b * a->hkv * s.own_tiles * s.own_splits + s.shared_items < INT_MAX, "grid too large");
+  SIG3D_REQUIRE(s.lds <= 152 * 1024, "bias table too large for LDS");
+  DecodeParams p = {};
+  p.q = a->q; p.table = a->table;
+  p.own = {a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->capacity};
+  p.shared = {a->shared_k, a->shared_v, a->shared_k_scale, a->shared_v_scale, a->shared_capacity};
+  p.lengths = a->lengths; p.shared_lengths = a->shared_lengths; p.counts = a->counts;
+  p.out = a->out; p.part = a->work;
+  p.q_b = a->q_b; p.q_n = a->q_n; p.q_h = a->q_h;
+  p.b = a->b; p.t = a->t; p.h = a->h; p.hkv = a->hkv; p.group = a->h / a->hkv;
+  p.each = a->groups ? a->b / a->groups : 0;
+  p.own_splits = s.own_splits; p.shared_splits = s.shared_splits; p.own_tiles = s.own_tiles; p.shared_tiles = s.shared_tiles;
+  p.shared_items = s.shared_items; p.bias_heads = s.bias_heads; p.joined = s.joined; p.direct = s.direct;
+  p.scale = a->scale;
+  p.bk = device_buckets(a->buckets);
+  return by_type(a->dtype, a->d, [&](auto t, auto d) {
+    typedef decltype(t) T;
+    constexpr int D = decltype(d)::value;
+    if (s.nb == 4) return quantized ? launch<T, D, true, 4>(p, s, (hipStream_t)stream) : launch<T, D, false, 4>(p, s, (hipStream_t)stream);
+    return quantized ? launch<T, D, true, 1>(p, s, (hipStream_t)stream) : launch<T, D, false, 1>(p, s, (hipStream_t)stream);
+  });
+}

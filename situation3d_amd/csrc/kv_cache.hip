@@ -1,0 +1,210 @@
+// kv_cache.hip -- writing the key / value cache, quantised on the way, and reading it back, for gfx950.
+//
+// A row is one (sequence, key head, token): d values.  Held as e4m3 it costs d bytes and one f32 scale, a power of two:
+//   scale = 2^e, e smallest with max |x| <= 448 * 2^e;   held = e4m3(x / scale), to nearest even.
+// With a power of two the quotient and the value read back are exact, so writing a value that came out of the cache gives it
+// again, and the 4 significant bits are the only rounding (half a step: 2^-4 of the value).
+//
+// Both directions move bytes and do next to no arithmetic: HBM bound.  The cache is head-major, (b, hkv, capacity, d), so
+// that a decoding workgroup streams one contiguous run; tokens arrive and leave token-major.  Work is ordered (sequence,
+// head, token): cache traffic is contiguous, and the token-major side moves whole rows of d elements (128 bytes and more).
+#include "lang_core.h"
+
+namespace {
+using namespace lang;
+
+struct AppendParams {
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  const int *start, *counts;
+  int *lengths;
+  long k_b, k_n, k_h, v_b, v_n, v_h;
+  int t, capacity, hkv;
+};
+
+// Four lanes hold a row, lane l the 16-byte pieces l, l + 4, ...
+template <typename T, int D> struct Row {
+  static constexpr int PER = 16 / (int)sizeof(T), N = D / PER / 4;
+  typedef T piece __attribute__((ext_vector_type(PER)));
+  piece x[N];
+  __device__ __forceinline__ void load(const T *row, int l) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const piece *>(row + (l + 4 * i) * PER);
+  }
+  __device__ __forceinline__ void put(T *row, int l) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<piece *>(row + (l + 4 * i) * PER) = x[i];
+  }
+  // the scale's exponent: infinities and NaN do not count
+  __device__ __forceinline__ int exponent() const {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const float a = fabsf((float)x[i][e]);
+        top = a < INFINITY ? fmaxf(top, a) : top;
+      }
+    top = fmaxf(top, __builtin_bit_cast(float, dpp_i32<0xB1>(__builtin_bit_cast(int, top))));
+    top = fmaxf(top, __builtin_bit_cast(float, dpp_i32<0x4E>(__builtin_bit_cast(int, top))));
+    // top = m 2^x with m in [0.5, 1), 448 = 0.875 2^9; scales stay normal numbers
+    const int ex = __builtin_amdgcn_frexp_expf(top) - 9 + (__builtin_amdgcn_frexp_mantf(top) > 0.875f ? 1 : 0);
+    return top > 0.f ? max(ex, -126) : 0;
+  }
+  __device__ __forceinline__ void put_e4m3(unsigned char *row, int l, int exponent) const {
+    const float inv = __builtin_ldexpf(1.f, -exponent);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      unsigned w[PER / 4];
+#pragma unroll
+      for (int g = 0; g < PER / 4; ++g) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = (float)x[i][4 * g + e] * inv;
+          y[e] = fabsf(y[e]) > 448.f ? copysignf(448.f, y[e]) : y[e];      // infinities; NaN stays
+        }
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        p = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], p, true);
+        w[g] = (unsigned)p;
+      }
+      unsigned *to = reinterpret_cast<unsigned *>(row + (l + 4 * i) * PER);
+      if constexpr (PER == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[PER / 4 - 1]);
+      else to[0] = w[0];
+    }
+  }
+};
+
+// grid (blocks of rows, b).  One block a sequence, or `start` given: lengths is updated here, after everyone has read it.
+template <typename T, int D, bool Q>
+__global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p) {
+  const int b = blockIdx.y, l = threadIdx.x & 3, rows = p.hkv * p.t;
+  const int first = p.start ? p.start[b] : p.lengths[b];
+  const int count = p.counts ? min(max(p.counts[b], 0), p.t) : p.t;
+  for (int r = blockIdx.x * 64 + (threadIdx.x >> 2); r < rows; r += gridDim.x * 64) {
+    const int head = r / p.t, i = r - head * p.t;
+    const long to = (long)first + i;
+    if (i >= count || to < 0 || to >= p.capacity) continue;        // the four lanes of a row agree
+    Row<T, D> k, v;
+    k.load(reinterpret_cast<const T *>(p.k) + b * p.k_b + i * p.k_n + head * p.k_h, l);
+    v.load(reinterpret_cast<const T *>(p.v) + b * p.v_b + i * p.v_n + head * p.v_h, l);
+    const long row = ((long)b * p.hkv + head) * p.capacity + to;
+    if constexpr (Q) {
+      const int ek = k.exponent(), ev = v.exponent();
+      k.put_e4m3(reinterpret_cast<unsigned char *>(p.k_cache) + row * D, l, ek);
+      v.put_e4m3(reinterpret_cast<unsigned char *>(p.v_cache) + row * D, l, ev);
+      if (l == 0) {
+        p.k_scale[row] = __builtin_ldexpf(1.f, ek);
+        p.v_scale[row] = __builtin_ldexpf(1.f, ev);
+      }
+    } else {
+      k.put(reinterpret_cast<T *>(p.k_cache) + row * D, l);
+      v.put(reinterpret_cast<T *>(p.v_cache) + row * D, l);
+    }
+  }
+  if (gridDim.x == 1 || p.start) {
+    __syncthreads();
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.lengths[b] = (int)min(max((long)first + count, 0l), (long)p.capacity);
+  }
+}
+
+__global__ __launch_bounds__(256) void cache_advance_kernel(int b, int t, int capacity, const int *counts, int *lengths) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= b) return;
+  const int count = counts ? min(max(counts[i], 0), t) : t;
+  lengths[i] = (int)min(max((long)lengths[i] + count, 0l), (long)capacity);
+}
+
+struct ReadParams {
+  const void *k, *v;
+  const float *k_scale, *v_scale;
+  const int *lengths;
+  void *k_out, *v_out;
+  int n, capacity, hkv;
+};
+
+// a thread: eight elements of a K row and of the V row beside it.  grid (n * D / 8 / 256, hkv, b)
+template <typename T, int D, bool Q>
+__global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
+  const int c = blockIdx.x * 256 + threadIdx.x, i = c / (D / 8), o = c - i * (D / 8);
+  if (i >= p.n) return;
+  const int b = blockIdx.z, head = blockIdx.y;
+  frag_t<T> k{}, v{};
+  if (i < p.lengths[b]) {
+    const long row = ((long)b * p.hkv + head) * p.capacity + i;
+    if constexpr (Q) {
+      const uint2 wk = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(p.k) + row * D + 8 * o);
+      const uint2 wv = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(p.v) + row * D + 8 * o);
+      k = from_e4m3<T>(wk, p.k_scale[row]);
+      v = from_e4m3<T>(wv, p.v_scale[row]);
+    } else {
+      k = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.k) + row * D + 8 * o);
+      v = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.v) + row * D + 8 * o);
+    }
+  }
+  const long to = (((long)b * p.n + i) * p.hkv + head) * D + 8 * o;
+  *reinterpret_cast<frag_t<T> *>(reinterpret_cast<T *>(p.k_out) + to) = k;
+  *reinterpret_cast<frag_t<T> *>(reinterpret_cast<T *>(p.v_out) + to) = v;
+}
+
+int check_cache(const char *where, int dtype, int b, int capacity, int hkv, int d) {
+  LANG_NEED(where, dtype >= 0 && dtype <= 2, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+  LANG_NEED(where, d == 64 || d == 96 || d == 128, "head size must be 64, 96 or 128");
+  LANG_NEED(where, b >= 1 && b <= 65535 && hkv >= 1 && hkv <= 65535 && capacity >= 1, "sizes out of range");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int sig3d_cache_append(const sig3d_cache_append_args *a, void *stream) {
+  SIG3D_REQUIRE(a != nullptr, "no arguments");
+  if (int e = check_cache("sig3d_cache_append", a->dtype, a->b, a->capacity, a->hkv, a->d)) return e;
+  SIG3D_REQUIRE(a->t >= 1 && (long)a->t * a->hkv < (1l << 30), "token count out of range");
+  SIG3D_REQUIRE(a->k && a->v && a->k_cache && a->v_cache && a->lengths, "missing array");
+  SIG3D_REQUIRE((a->k_scale == nullptr) == (a->v_scale == nullptr), "k_scale and v_scale come together");
+  SIG3D_REQUIRE(aligned16(a->k) && aligned16(a->v) && aligned16(a->k_cache) && aligned16(a->v_cache),
+                "addresses must be 16-byte aligned");
+  const int e = a->dtype == 0 ? 4 : 2;
+  const long strides[6] = {a->k_b, a->k_n, a->k_h, a->v_b, a->v_n, a->v_h};
+  for (long s : strides) SIG3D_REQUIRE(s >= 0 && s * e % 16 == 0, "strides must be non-negative multiples of 16 bytes");
+  const AppendParams p = {a->k, a->v, a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->start, a->counts, a->lengths,
+                          a->k_b, a->k_n, a->k_h, a->v_b, a->v_n, a->v_h, a->t, a->capacity, a->hkv};
+  const int rows = a->hkv * a->t;
+  // without `start` every workgroup of a sequence reads the length that the call moves: one workgroup up to 512 rows (a
+  // decoding step: 32 heads are half a pass), else a launch of its own moves it
+  const bool one = !a->start && rows <= 512;
+  const dim3 grid(one ? 1 : sig3d_ceil_div(rows, 64), a->b);
+  const int err = by_type(a->dtype, a->d, [&](auto t, auto d) {
+    typedef decltype(t) T;
+    constexpr int D = decltype(d)::value;
+    if (a->k_scale) cache_append_kernel<T, D, true><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+    else cache_append_kernel<T, D, false><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+    SIG3D_LAUNCH_CHECK("cache_append_kernel");
+    return 0;
+  });
+  if (err || grid.x == 1 || a->start) return err;
+  cache_advance_kernel<<<sig3d_ceil_div(a->b, 256), 256, 0, (hipStream_t)stream>>>(a->b, a->t, a->capacity, a->counts, a->lengths);
+  SIG3D_LAUNCH_CHECK("cache_advance_kernel");
+  return 0;
+}
+
+extern "C" int sig3d_cache_read(int dtype, int b, int n, int capacity, int hkv, int d, const void *k_cache, const void *v_cache,
+                                const float *k_scale, const float *v_scale, const int *lengths, void *k_out, void *v_out,
+                                void *stream) {
+  if (int e = check_cache("sig3d_cache_read", dtype, b, capacity, hkv, d)) return e;
+  SIG3D_REQUIRE(n >= 1 && n <= capacity && (long)n * d < (1l << 33), "row count out of range");
+  SIG3D_REQUIRE(k_cache && v_cache && lengths && k_out && v_out, "missing array");
+  SIG3D_REQUIRE((k_scale == nullptr) == (v_scale == nullptr), "k_scale and v_scale come together");
+  SIG3D_REQUIRE(aligned16(k_cache) && aligned16(v_cache) && aligned16(k_out) && aligned16(v_out), "addresses must be 16-byte aligned");
+  const ReadParams p = {k_cache, v_cache, k_scale, v_scale, lengths, k_out, v_out, n, capacity, hkv};
+  const dim3 grid(sig3d_ceil_div((long)n * (d / 8), 256), hkv, b);
+  return by_type(dtype, d, [&](auto t, auto dd) {
+    typedef decltype(t) T;
+    constexpr int D = decltype(dd)::value;
+    if (k_scale) cache_read_kernel<T, D, true><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+    else cache_read_kernel<T, D, false><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+    SIG3D_LAUNCH_CHECK("cache_read_kernel");
+    return 0;
+  });
+}

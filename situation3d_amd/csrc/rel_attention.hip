@@ -1,0 +1,777 @@
+// rel_attention.hip -- attention with a learned relative position bias, forward and backward, for gfx950.
+//
+//   s_ij = scale q_i.k_j + table[bucket(j - p_i)][head],  p_i = i + query_offset,  o_i = softmax(s_i) V
+// over the keys that query i sees; scores, probabilities and the bias matrix never leave the chip.  The reference
+// (modeling_t5.py's attention) materialises the (b, h, nq, nk) bias, scores and probabilities.
+//
+// What a query sees is always ONE interval [lo, hi) of keys -- key lengths, causal and prefix masks and packed documents are
+// all intervals -- so masks cost two integers a row, and whole tiles are classified by four: outside (skipped), inside
+// (no mask code), or cut.
+//
+// The bias is a function of the distance alone and constant from `reach` on: a workgroup keeps log2(e) * bias for the
+// 2 reach + 1 distances in LDS; tiles wholly beyond `reach` add one constant, the few along the diagonal gather.
+//
+// Statistics, accumulators, the running maximum and sum are f32.  P and dS are rounded to the operand type where they become
+// an operand of the next product (bf16 / f16 matrix instructions take nothing else; f32 stays f32).  f16 has no exponents to
+// spare for that -- P is 1 / nk on average, gradients are small -- so its backward pass holds 2^8 P and dS times the power of
+// two that brings the largest |dO| (of the query for dQ, of the sequence's queries for dK) to [4, 8), and takes both back out
+// of the f32 sums.
+#include "lang_core.h"
+
+#include <limits.h>
+
+namespace {
+using namespace lang;
+
+struct Params {
+  const void *q, *k, *v, *table, *grad;
+  const int *key_lengths, *prefix_lengths, *key_ranges;
+  void *out, *dq, *dk, *dv, *dtable;
+  float *out32, *lse, *delta, *hist;
+  int4 *blocks;                               // backward: interval summary of every 32 queries
+  int *tops;                                  // backward, f16: exponent of the largest |dO| of a head's 32 queries
+  long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, grad_b, grad_n, grad_h;
+  int b, nq, nk, h, hkv, group, causal, offset, table_rows, qtiles, ktiles;
+  float scale;
+  Buckets bk;
+};
+
+// The keys [lo, hi) that query i of sequence b sees; lo = hi = 0 for none.
+__device__ __forceinline__ void interval(const Params &p, int b, int i, int &lo, int &hi) {
+  lo = 0;
+  hi = p.nk;
+  if (p.key_lengths) hi = min(hi, p.key_lengths[b]);
+  if (p.causal) {
+    long seen = (long)i + p.offset + 1;
+    if (p.prefix_lengths) seen = max(seen, (long)p.prefix_lengths[b]);
+    hi = (int)min((long)hi, seen);
+  }
+  if (p.key_ranges) {
+    const int2 r = reinterpret_cast<const int2 *>(p.key_ranges)[(long)b * p.nq + i];
+    lo = max(lo, r.x);
+    hi = min(hi, r.y);
+  }
+  if (lo >= hi) lo = hi = 0;
+}
+
+// What 32 queries see together: any = the union's ends, all = the interval that every one of them sees whole.
+struct Span { int any_lo, any_hi, all_lo, all_hi; };
+__device__ __forceinline__ Span span_of(int lo, int hi, bool valid) {
+  Span s;
+  s.any_lo = wave_min_i32(valid && lo < hi ? lo : INT_MAX);
+  s.any_hi = wave_max_i32(valid && lo < hi ? hi : 0);
+  s.all_lo = wave_max_i32(valid ? lo : 0);
+  s.all_hi = wave_min_i32(valid ? hi : INT_MAX);
+  return s;
+}
+
+// Consecutive workgroups go to the 8 XCDs in turn; give each XCD a contiguous share of the work instead, so that the
+// workgroups that read the same keys share an L2.
+__device__ __forceinline__ int xcd_contiguous(int id, int total) {
+  const int each = total >> 3;
+  return id < each * 8 ? (id & 7) * each + (id >> 3) : id;
+}
+
+// Rows [row0, row0 + ROWS) of a token-major operand through registers into an LDS tile; rows outside [lo, hi) become zero.
+template <typename T, int D, int ROWS, int NT> struct Stage {
+  typedef Tile<T, D> TL;
+  static constexpr int N = (ROWS * TL::CH + NT - 1) / NT;
+  u32x4 r[N];
+  __device__ __forceinline__ void load(const T *base, long stride, int row0, int lo, int hi, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + i * NT, row = c / TL::CH, ch = c - row * TL::CH;
+      r[i] = u32x4{0, 0, 0, 0};
+      if ((ROWS * TL::CH % NT == 0 || row < ROWS) && row0 + row >= lo && row0 + row < hi)
+        r[i] = *reinterpret_cast<const u32x4 *>(base + (long)(row0 + row) * stride + ch * (16 / (int)sizeof(T)));
+    }
+  }
+  __device__ __forceinline__ void store(char *tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + i * NT, row = c / TL::CH, ch = c - row * TL::CH;
+      if (ROWS * TL::CH % NT == 0 || row < ROWS) *reinterpret_cast<u32x4 *>(tile + TL::at(row, ch)) = r[i];
+    }
+  }
+};
+
+// fragment f of a stationary row: elements 16 f + 8 half .. + 7; zero when the row does not exist
+template <typename T, int D>
+__device__ __forceinline__ void load_row(frag_t<T> (&f)[D / 16], const T *row, int half, bool valid) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    frag_t<T> x{};
+    if (valid) x = *reinterpret_cast<const frag_t<T> *>(row + 16 * s + 8 * half);
+    f[s] = x;
+  }
+}
+
+// A (D x 32) accumulator whose columns are rows of a dense tensor: registers 4 g .. 4 g + 3 are four consecutive elements.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(T *row, const f32x16 (&acc)[D / 32], float factor, int half) {
+#pragma unroll
+  for (int blk = 0; blk < D / 32; ++blk)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = acc[blk][4 * g + e] * factor;
+      *reinterpret_cast<vec4_t<T> *>(row + 32 * blk + 8 * g + 4 * half) = to_vec4<T>(x);
+    }
+}
+
+template <typename T> constexpr bool narrow() { return std::is_same<T, _Float16>::value; }
+constexpr int P_UP = 8, DS_UP = 3;            // f16: exponents that P and dS are raised by (see the top)
+
+template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+
+// s (scaled scores of a 32 x 32 block, in log2 units) += bias.  first = position of register 0's row minus that of the lane's
+// column, i.e. register r stands at relative position first + sign * (16 (r >> 3) + (r & 7)).
+template <int SIGN>
+__device__ __forceinline__ void add_bias(f32x16 &s, const float *by_distance, int reach, int first) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int rel = first + SIGN * (16 * (r >> 3) + (r & 7));
+    s[r] += by_distance[min(max(rel, -reach), reach) + reach];
+  }
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------
+// A wave owns 32 queries (columns), a workgroup NW waves that share the streamed key tiles in a double-buffered LDS pair:
+// the next tile's loads are in flight while the current one is used, one barrier a tile.
+// S^T = K Q^T, then O^T = V^T P^T: a query is one lane (and lane ^ 32), its softmax is in-lane work.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
+  typedef Tile<T, D> TL;
+  constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
+  extern __shared__ __align__(16) char lds[];
+  float *bias = reinterpret_cast<float *>(lds + 4 * TB);
+  __shared__ int ends[2][NW];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;      // causal: the long rows first
+  const int b = bh / p.h, head = bh - b * p.h;
+  const int qi = (qt * NW + wave) * 32 + col;
+  const bool valid = qi < p.nq;
+  int lo = 0, hi = 0;
+  if (valid) interval(p, b, qi, lo, hi);
+  const Span sp = span_of(lo, hi, valid);
+  if (lane == 0) {
+    ends[0][wave] = sp.any_lo;
+    ends[1][wave] = sp.any_hi;
+  }
+  frag_t<T> qf[D / 16];
+  load_row<T, D>(qf, reinterpret_cast<const T *>(p.q) + b * p.q_b + (long)qi * p.q_n + head * p.q_h, half, valid);
+  const bool biased = p.bk.n > 0;
+  if (biased) fill_bias(bias, p.bk, reinterpret_cast<const T *>(p.table), p.h, head, tid, NT);
+  __syncthreads();
+  int wlo = INT_MAX, whi = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    wlo = min(wlo, ends[0][w]);
+    whi = max(whi, ends[1][w]);
+  }
+  const int kvh = head / p.group;
+  const T *kb = reinterpret_cast<const T *>(p.k) + b * p.k_b + kvh * p.k_h;
+  const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
+  const float scale2 = p.scale * LOG2E;
+  const int reach = p.bk.reach, qpos = qi + p.offset, q0pos = (qt * NW + wave) * 32 + p.offset;
+
+  f32x16 o[D / 32] = {};
+  float m = -INFINITY, l = 0.f;
+  const int first = wlo < whi ? wlo / KT * KT : 0;
+  Stage<T, D, KT, NT> ks, vs;
+  if (wlo < whi) {
+    ks.load(kb, p.k_n, first, wlo, whi, tid);
+    vs.load(vb, p.v_n, first, wlo, whi, tid);
+    ks.store(lds, tid);
+    vs.store(lds + TB, tid);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int t = first; t < whi; t += KT, buf ^= 1) {
+    const bool more = t + KT < whi;
+    if (more) {
+      ks.load(kb, p.k_n, t + KT, wlo, whi, tid);
+      vs.load(vb, p.v_n, t + KT, wlo, whi, tid);
+    }
+    if (t < sp.any_hi && t + KT > sp.any_lo) {
+      const char *kt = lds + buf * 2 * TB, *vt = kt + TB;
+      f32x16 s[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        s[u] = f32x16{};
+#pragma unroll
+        for (int f = 0; f < D / 16; ++f)
+          s[u] = mma32(TL::row_frag(kt, u * 32 + kappa(col), 2 * f + half), qf[f], s[u]);
+      }
+      float add = 0.f;
+      bool near = false;
+      if (biased) {
+        const int nearest_lo = t - (q0pos + 31), nearest_hi = t + KT - 1 - q0pos;
+        near = nearest_hi > -reach && nearest_lo < reach;
+        if (!near) add = nearest_hi <= -reach ? bias[0] : bias[2 * reach];
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], scale2, add);
+        if (near) add_bias<1>(s[u], bias, reach, t + u * 32 + 8 * half - qpos);
+      }
+      if (t < sp.all_lo || t + KT > sp.all_hi) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if ((unsigned)(t + u * 32 + reg_row(r, half) - lo) >= (unsigned)(hi - lo)) s[u][r] = -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+      top = max_halves(top);
+      if (__any(top > m)) {                                  // the running maximum rarely moves after the first tiles
+        const float now = fmaxf(m, top);
+        const float keep = now == -INFINITY ? 1.f : exp2_(m - now);
+        m = now;
+        l *= keep;
+#pragma unroll
+        for (int blk = 0; blk < D / 32; ++blk)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[blk][r] *= keep;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[u][r] = exp2_(s[u][r] - base);
+          l += s[u][r];
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          f32x8 x;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = s[u][8 * g + j];
+          const frag_t<T> pf = to_frag<T>(x);
+#pragma unroll
+          for (int blk = 0; blk < D / 32; ++blk)
+            o[blk] = mma32(TL::col_frag(vt, u * 32 + 16 * g + 8 * half, 32 * blk + (lane & 16), lane), pf, o[blk]);
+        }
+      }
+    }
+    if (more) {
+      ks.store(lds + (buf ^ 1) * 2 * TB, tid);
+      vs.store(lds + (buf ^ 1) * 2 * TB + TB, tid);
+    }
+    __syncthreads();
+  }
+  if (!valid) return;
+  l = sum_halves(l);
+  const bool empty = lo >= hi;
+  const float inv = empty ? 0.f : 1.f / l;
+  const long row = (((long)b * p.nq + qi) * p.h + head) * D;
+  store_row<T, D>(reinterpret_cast<T *>(p.out) + row, o, inv, half);
+  if (p.out32) {
+    store_row<float, D>(p.out32 + row, o, inv, half);
+    if (half == 0) p.lse[((long)b * p.h + head) * p.nq + qi] = empty ? INFINITY : m + __builtin_amdgcn_logf(l);
+  }
+}
+
+// ---- backward: dQ, delta, the table's gradient ------------------------------------------------------------------------------
+// Same tiling as the forward pass (a query is a lane): P = exp2(s - lse), dP^T = V dO^T, dS = P (dP - delta) with
+// delta = dO.O from the unrounded O, dQ^T = K^T dS^T.
+// Table: dS summed by distance.  Beyond `reach` everything falls into the end buckets: two registers.  Along the diagonal
+// each wave adds its dS into its own LDS row of 2 reach + 1 distances; one instruction adds the 32 lanes of one half, whose
+// distances differ, so no two lanes meet at an address and the order of the sums is that of the program.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
+  typedef Tile<T, D> TL;
+  constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
+  extern __shared__ __align__(16) char lds[];
+  float *bias = reinterpret_cast<float *>(lds + 4 * TB);
+  const int reach = p.bk.reach, span = 2 * reach + 1;
+  float *sums = bias + span;                              // [NW][span]
+  __shared__ int ends[2][NW];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;
+  const int b = bh / p.h, head = bh - b * p.h;
+  const int qi = (qt * NW + wave) * 32 + col;
+  const bool valid = qi < p.nq;
+  int lo = 0, hi = 0;
+  if (valid) interval(p, b, qi, lo, hi);
+  const Span sp = span_of(lo, hi, valid);
+  if (lane == 0) {
+    ends[0][wave] = sp.any_lo;
+    ends[1][wave] = sp.any_hi;
+    if (head == 0) p.blocks[((long)b * p.qtiles + qt) * NW + wave] = make_int4(sp.any_lo, sp.any_hi, sp.all_lo, sp.all_hi);
+  }
+  frag_t<T> qf[D / 16], gf[D / 16];
+  load_row<T, D>(qf, reinterpret_cast<const T *>(p.q) + b * p.q_b + (long)qi * p.q_n + head * p.q_h, half, valid);
+  load_row<T, D>(gf, reinterpret_cast<const T *>(p.grad) + b * p.grad_b + (long)qi * p.grad_n + head * p.grad_h, half, valid);
+  const long row = (((long)b * p.nq + qi) * p.h + head) * D, stat = ((long)b * p.h + head) * p.nq + qi;
+  float delta = 0.f, lse = INFINITY;
+  if (valid) {
+    lse = p.lse[stat];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const f32x8 x = *reinterpret_cast<const f32x8 *>(p.out32 + row + 16 * s + 8 * half);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[s][j], x[j], delta);
+    }
+  }
+  delta = sum_halves(delta);
+  if (valid && half == 0) p.delta[stat] = delta;
+  float undo = 1.f;                                       // dS is held times 1 / undo
+  if constexpr (narrow<T>()) {
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf((float)gf[s][j]));
+    top = max_halves(top);
+    const bool plain = !(top > 0.f && top < INFINITY);
+    const int e = plain ? DS_UP : __builtin_amdgcn_frexp_expf(top);      // top in [2^(e-1), 2^e)
+    undo = __builtin_ldexpf(1.f, e - DS_UP);
+    lse += (float)(e - DS_UP);
+    const int most = wave_max_i32(plain ? -64 : e);
+    if (lane == 0) p.tops[((long)bh * p.qtiles + qt) * NW + wave] = most;
+  }
+  const bool biased = p.bk.n > 0;
+  if (biased) {
+    fill_bias(bias, p.bk, reinterpret_cast<const T *>(p.table), p.h, head, tid, NT);
+    for (int i = tid; i < NW * span; i += NT) sums[i] = 0.f;
+  }
+  __syncthreads();
+  int wlo = INT_MAX, whi = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    wlo = min(wlo, ends[0][w]);
+    whi = max(whi, ends[1][w]);
+  }
+  const int kvh = head / p.group;
+  const T *kb = reinterpret_cast<const T *>(p.k) + b * p.k_b + kvh * p.k_h;
+  const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
+  const float scale2 = p.scale * LOG2E;
+  const int qpos = qi + p.offset, q0pos = (qt * NW + wave) * 32 + p.offset;
+  float *mine = sums + wave * span;
+
+  f32x16 dq[D / 32] = {};
+  float behind = 0.f, ahead = 0.f;
+  const int first = wlo < whi ? wlo / KT * KT : 0;
+  Stage<T, D, KT, NT> ks, vs;
+  if (wlo < whi) {
+    ks.load(kb, p.k_n, first, wlo, whi, tid);
+    vs.load(vb, p.v_n, first, wlo, whi, tid);
+    ks.store(lds, tid);
+    vs.store(lds + TB, tid);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int t = first; t < whi; t += KT, buf ^= 1) {
+    const bool more = t + KT < whi;
+    if (more) {
+      ks.load(kb, p.k_n, t + KT, wlo, whi, tid);
+      vs.load(vb, p.v_n, t + KT, wlo, whi, tid);
+    }
+    if (t < sp.any_hi && t + KT > sp.any_lo) {
+      const char *kt = lds + buf * 2 * TB, *vt = kt + TB;
+      const bool cut = t < sp.all_lo || t + KT > sp.all_hi;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        f32x16 s{}, dp{};
+#pragma unroll
+        for (int f = 0; f < D / 16; ++f) {
+          s = mma32(TL::row_frag(kt, u * 32 + kappa(col), 2 * f + half), qf[f], s);
+          dp = mma32(TL::row_frag(vt, u * 32 + kappa(col), 2 * f + half), gf[f], dp);
+        }
+        float add = 0.f;
+        bool near = false, left = false;
+        if (biased) {
+          const int nearest_lo = t + u * 32 - (q0pos + 31), nearest_hi = t + u * 32 + 31 - q0pos;
+          left = nearest_hi <= -reach;
+          near = !left && nearest_lo < reach;
+          if (!near) add = left ? bias[0] : bias[2 * reach];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, add);
+        const int rel0 = t + u * 32 + 8 * half - qpos;
+        if (near) add_bias<1>(s, bias, reach, rel0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = exp2_(s[r] - lse) * (dp[r] - delta);
+        }
+        if (cut) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if ((unsigned)(t + u * 32 + reg_row(r, half) - lo) >= (unsigned)(hi - lo)) s[r] = 0.f;
+        }
+        if (biased) {
+          if (near) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int rel = rel0 + 16 * (r >> 3) + (r & 7);
+              if (rel <= -reach) behind += s[r] * undo;
+              else if (rel >= reach) ahead += s[r] * undo;
+              else {
+                if (half == 0) __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float *)(mine + rel + reach), s[r] * undo, 0, 0, false);
+                if (half == 1) __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float *)(mine + rel + reach), s[r] * undo, 0, 0, false);
+              }
+            }
+          } else {
+            float x = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x += s[r];
+            (left ? behind : ahead) += x * undo;
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          f32x8 x;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = s[8 * g + j];
+          const frag_t<T> df = to_frag<T>(x);
+#pragma unroll
+          for (int blk = 0; blk < D / 32; ++blk)
+            dq[blk] = mma32(TL::col_frag(kt, u * 32 + 16 * g + 8 * half, 32 * blk + (lane & 16), lane), df, dq[blk]);
+        }
+      }
+    }
+    if (more) {
+      ks.store(lds + (buf ^ 1) * 2 * TB, tid);
+      vs.store(lds + (buf ^ 1) * 2 * TB + TB, tid);
+    }
+    __syncthreads();
+  }
+  if (valid) store_row<T, D>(reinterpret_cast<T *>(p.dq) + row, dq, p.scale * undo, half);
+  if (!biased) return;
+  const float far_behind = wave_allreduce_sum_f32(behind), far_ahead = wave_allreduce_sum_f32(ahead);
+  if (lane == 0) {
+    mine[0] += far_behind;
+    mine[2 * reach] += far_ahead;
+  }
+  __syncthreads();
+  // distances -> buckets (keys ahead share bucket 0 unless they have their own), one row of partial sums a workgroup
+  float *part = p.hist + ((long)bh * p.qtiles + qt) * p.table_rows;
+  for (int bucket = tid; bucket < p.table_rows; bucket += NT) {
+    float x = 0.f;
+    const bool second = p.bk.both && bucket >= p.bk.n && bucket < 2 * p.bk.n, first_dir = bucket < p.bk.n;
+    if (first_dir || second) {
+      const int i = second ? bucket - p.bk.n : bucket;
+      const int from = p.bk.border[i], to = i + 1 < p.bk.n ? p.bk.border[i + 1] : reach + 1;      // distances [from, to)
+      for (int a = from; a < to; ++a) {
+        if (second ? a == 0 : false) continue;
+        const int at = second ? reach + a : reach - a;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) x += sums[w * span + at];
+      }
+      if (!second && !p.bk.both && i == 0)
+        for (int a = 1; a <= reach; ++a)
+#pragma unroll
+          for (int w = 0; w < NW; ++w) x += sums[w * span + reach + a];
+    }
+    part[bucket] = x;
+  }
+}
+
+// table gradient: partial rows (b, head, query tile) -> (rows, h), summed in f32 in a fixed order
+template <typename T>
+__global__ __launch_bounds__(256) void rel_bwd_table_kernel(const float *hist, int b, int h, int qtiles, int rows, T *dtable) {
+  const int head = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int bucket = blockIdx.y * 4 + wave; bucket < rows; bucket += 4 * gridDim.y) {
+    float x = 0.f;
+    const int n = b * qtiles;
+    for (int i = lane; i < n; i += 64) {
+      const int bi = i / qtiles, qt = i - bi * qtiles;
+      x += hist[(((long)bi * h + head) * qtiles + qt) * rows + bucket];
+    }
+    x = wave_allreduce_sum_f32(x);
+    if (lane == 0) dtable[(long)bucket * h + head] = (T)x;
+  }
+}
+
+// ---- backward: dK, dV --------------------------------------------------------------------------------------------------------
+// A wave owns 32 keys (columns; K and V rows in registers), a workgroup NW waves that share the streamed query tiles (Q, dO,
+// lse, delta, intervals).  S = Q K^T, dP = dO V^T with queries along the registers: P and dS are at once the B operands of
+// dV^T += dO^T P and dK^T += Q^T dS.  The heads that share the keys are a loop: their sums stay in the accumulators.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void rel_bwd_dkv_kernel(const Params p) {
+  typedef Tile<T, D> TL;
+  constexpr int QT = key_tile<T>(), NT = NW * 64, SUB = QT / 32, TB = QT * TL::ROW;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ float stats[2][2][QT];            // [buffer][lse, delta]
+  __shared__ int rows[2][2][QT];               // [buffer][lo, hi]
+  __shared__ int todo[256], ntodo;
+  float *bias = reinterpret_cast<float *>(lds + 4 * TB);
+  const int reach = p.bk.reach;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int bh = id / p.ktiles, kt0 = id % p.ktiles;
+  const int b = bh / p.hkv, kvh = bh - b * p.hkv;
+  const int k0 = kt0 * NW * 32, kw = k0 + wave * 32, key = kw + col;
+  const bool valid = key < p.nk;
+  frag_t<T> kf[D / 16], vf[D / 16];
+  load_row<T, D>(kf, reinterpret_cast<const T *>(p.k) + b * p.k_b + (long)key * p.k_n + kvh * p.k_h, half, valid);
+  load_row<T, D>(vf, reinterpret_cast<const T *>(p.v) + b * p.v_b + (long)key * p.v_n + kvh * p.v_h, half, valid);
+  const bool biased = p.bk.n > 0;
+  const float scale2 = p.scale * LOG2E;
+  const int nblocks = (p.nq + 31) / 32, ntiles = (p.nq + QT - 1) / QT;
+  const int4 *blocks = p.blocks + (long)b * ((p.nq + 32 * 4 - 1) / (32 * 4)) * 4;
+
+  int up = 0;                                  // f16: dS is held times 2^up, P times 2^P_UP
+  if constexpr (narrow<T>()) {
+    int most = -64;
+    for (int i = tid; i < p.group * nblocks; i += NT) {
+      const int hh = i / nblocks, blk = i - hh * nblocks;
+      most = max(most, p.tops[((long)b * p.h + kvh * p.group + hh) * p.qtiles * NW + blk]);
+    }
+    most = wave_max_i32(most);
+    if (lane == 0) todo[wave] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) most = max(most, todo[w]);
+    up = most == -64 ? 0 : DS_UP - most;
+  }
+  const float ds_factor = __builtin_ldexpf(1.f, up - (narrow<T>() ? P_UP : 0));
+
+  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+  for (int head = kvh * p.group; head < (kvh + 1) * p.group; ++head) {
+    if (biased) {
+      __syncthreads();
+      fill_bias(bias, p.bk, reinterpret_cast<const T *>(p.table), p.h, head, tid, NT);
+    }
+    const T *qb = reinterpret_cast<const T *>(p.q) + b * p.q_b + head * p.q_h;
+    const T *gb = reinterpret_cast<const T *>(p.grad) + b * p.grad_b + head * p.grad_h;
+    const long stat = ((long)b * p.h + head) * p.nq;
+    for (int chunk = 0; chunk < ntiles; chunk += 256) {
+      // query tiles that see any of these keys, in order; bit 30: some query does not see all of them
+      __syncthreads();
+      if (wave == 0) {
+        int n = 0;
+        for (int c = chunk; c < min(chunk + 256, ntiles); c += 64) {
+          const int tile = c + lane;
+          bool any = false, cut = false;
+          if (tile < ntiles) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+              const int blk = tile * SUB + u;
+              if (blk >= nblocks) continue;
+              const int4 s = blocks[blk];
+              any |= s.x < k0 + NW * 32 && s.y > k0;
+              cut |= s.z > k0 || s.w < min(k0 + NW * 32, p.nk);
+            }
+          }
+          const unsigned long long mask = __ballot(any);
+          if (any) todo[n + __popcll(mask & ((1ull << lane) - 1))] = tile | (cut ? 1 << 30 : 0);
+          n += __popcll(mask);
+        }
+        if (lane == 0) ntodo = n;
+      }
+      __syncthreads();
+      const int n = ntodo;
+      Stage<T, D, QT, NT> qs, gs;
+      float st = 0.f, dl = 0.f;
+      int rlo = 0, rhi = 0;
+      auto fetch = [&](int tile) {
+        const int q0 = tile * QT;
+        qs.load(qb, p.q_n, q0, 0, p.nq, tid);
+        gs.load(gb, p.grad_n, q0, 0, p.nq, tid);
+        if (tid < QT) {
+          const int qi = q0 + tid;
+          st = INFINITY; dl = 0.f; rlo = rhi = 0;
+          if (qi < p.nq) {
+            st = p.lse[stat + qi] - (narrow<T>() ? P_UP : 0);
+            dl = p.delta[stat + qi] * ds_factor;
+            interval(p, b, qi, rlo, rhi);
+          }
+        }
+      };
+      auto put = [&](int buf) {
+        qs.store(lds + buf * 2 * TB, tid);
+        gs.store(lds + buf * 2 * TB + TB, tid);
+        if (tid < QT) {
+          stats[buf][0][tid] = st; stats[buf][1][tid] = dl;
+          rows[buf][0][tid] = rlo; rows[buf][1][tid] = rhi - rlo;
+        }
+      };
+      if (n > 0) {
+        fetch(todo[0] & ~(1 << 30));
+        put(0);
+      }
+      __syncthreads();
+      for (int i = 0; i < n; ++i) {
+        const int buf = i & 1, entry = todo[i], q0 = (entry & ~(1 << 30)) * QT;
+        const bool cut = entry >> 30;
+        if (i + 1 < n) fetch(todo[i + 1] & ~(1 << 30));
+        const char *qt = lds + buf * 2 * TB, *gt = qt + TB;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          f32x16 s{}, dp{};
+#pragma unroll
+          for (int f = 0; f < D / 16; ++f) {
+            s = mma32(TL::row_frag(qt, u * 32 + kappa(col), 2 * f + half), kf[f], s);
+            dp = mma32(TL::row_frag(gt, u * 32 + kappa(col), 2 * f + half), vf[f], dp);
+          }
+          const int p0 = q0 + u * 32 + p.offset;
+          float add = 0.f;
+          bool near = false;
+          if (biased) {
+            const int nearest_lo = kw - (p0 + 31), nearest_hi = kw + 31 - p0;
+            near = nearest_hi > -reach && nearest_lo < reach;
+            if (!near) add = nearest_hi <= -reach ? bias[0] : bias[2 * reach];
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, add);
+          if (near) add_bias<-1>(s, bias, reach, key - (p0 + 8 * half));
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int at = u * 32 + 16 * g + 8 * half;
+            const f32x4 l0 = *reinterpret_cast<const f32x4 *>(&stats[buf][0][at]);
+            const f32x4 l1 = *reinterpret_cast<const f32x4 *>(&stats[buf][0][at + 4]);
+            const f32x4 d0 = *reinterpret_cast<const f32x4 *>(&stats[buf][1][at]);
+            const f32x4 d1 = *reinterpret_cast<const f32x4 *>(&stats[buf][1][at + 4]);
+            f32x8 x, y;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              x[j] = exp2_(s[8 * g + j] - (j < 4 ? l0[j & 3] : l1[j & 3]));
+              y[j] = x[j] * __builtin_fmaf(dp[8 * g + j], ds_factor, -(j < 4 ? d0[j & 3] : d1[j & 3]));
+            }
+            if (cut) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if ((unsigned)(key - rows[buf][0][at + j]) >= (unsigned)rows[buf][1][at + j]) x[j] = y[j] = 0.f;
+            }
+            const frag_t<T> pf = to_frag<T>(x), df = to_frag<T>(y);
+#pragma unroll
+            for (int blk = 0; blk < D / 32; ++blk) {
+              dv[blk] = mma32(TL::col_frag(gt, at, 32 * blk + (lane & 16), lane), pf, dv[blk]);
+              dk[blk] = mma32(TL::col_frag(qt, at, 32 * blk + (lane & 16), lane), df, dk[blk]);
+            }
+          }
+        }
+        if (i + 1 < n) put(buf ^ 1);
+        __syncthreads();
+      }
+    }
+  }
+  if (!valid) return;
+  const long row = (((long)b * p.nk + key) * p.hkv + kvh) * D;
+  store_row<T, D>(reinterpret_cast<T *>(p.dk) + row, dk, p.scale * __builtin_ldexpf(1.f, -up), half);
+  store_row<T, D>(reinterpret_cast<T *>(p.dv) + row, dv, narrow<T>() ? 1.f / (1 << P_UP) : 1.f, half);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------------------
+constexpr int NW = 4;                          // waves of a workgroup: 128 queries (forward, dQ) or keys (dK, dV)
+
+int check(const char *where, const sig3d_rel_attention_args *a) {
+  LANG_NEED(where, a != nullptr, "no arguments");
+  LANG_NEED(where, a->dtype >= 0 && a->dtype <= 2, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+  LANG_NEED(where, a->b >= 1 && a->nq >= 1 && a->nk >= 1 && a->h >= 1 && a->hkv >= 1, "sizes must be positive");
+  LANG_NEED(where, a->d == 64 || a->d == 96 || a->d == 128, "head size must be 64, 96 or 128");
+  LANG_NEED(where, a->h % a->hkv == 0, "heads must be a multiple of key heads");
+  LANG_NEED(where, a->nq <= (1 << 29) && a->nk <= (1 << 29), "at most 2^29 tokens");
+  LANG_NEED(where, a->query_offset > -(1 << 29) && a->query_offset < (1 << 29), "query_offset out of range");
+  const int e = a->dtype == 0 ? 4 : 2;
+  const long strides[9] = {a->q_b, a->q_n, a->q_h, a->k_b, a->k_n, a->k_h, a->v_b, a->v_n, a->v_h};
+  for (long s : strides) LANG_NEED(where, s >= 0 && s * e % 16 == 0, "strides must be non-negative multiples of 16 bytes");
+  LANG_NEED(where, a->q && a->k && a->v && a->out && aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->out),
+       "q, k, v, out must be 16-byte aligned addresses");
+  LANG_NEED(where, (a->out32 == nullptr) == (a->lse == nullptr) && aligned16(a->out32), "out32 and lse come together");
+  if (int e = check_buckets(where, a->buckets, a->table, a->table_rows)) return e;
+  LANG_NEED(where, (long)a->b * a->h * ((a->nq + 31) / 32) < INT_MAX && (long)a->b * a->h * ((a->nk + 31) / 32) < INT_MAX, "grid too large");
+  return 0;
+}
+
+Params params(const sig3d_rel_attention_args *a) {
+  Params p = {};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.table = a->table; p.grad = a->grad;
+  p.key_lengths = a->key_lengths; p.prefix_lengths = a->prefix_lengths; p.key_ranges = a->key_ranges;
+  p.out = a->out; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.dtable = a->dtable;
+  p.out32 = a->out32; p.lse = a->lse;
+  p.q_b = a->q_b; p.q_n = a->q_n; p.q_h = a->q_h; p.k_b = a->k_b; p.k_n = a->k_n; p.k_h = a->k_h;
+  p.v_b = a->v_b; p.v_n = a->v_n; p.v_h = a->v_h; p.grad_b = a->grad_b; p.grad_n = a->grad_n; p.grad_h = a->grad_h;
+  p.b = a->b; p.nq = a->nq; p.nk = a->nk; p.h = a->h; p.hkv = a->hkv; p.group = a->h / a->hkv;
+  p.causal = a->causal; p.offset = a->query_offset; p.table_rows = a->table_rows;
+  p.qtiles = sig3d_ceil_div(a->nq, NW * 32);
+  p.ktiles = sig3d_ceil_div(a->nk, NW * 32);
+  p.scale = a->scale;
+  p.bk = device_buckets(a->buckets);
+  return p;
+}
+
+// workspace of the backward pass: delta (b h nq), interval summaries (b, 4 per 128 queries) int4, exponents of |dO| (f16),
+// partial table gradients
+long work_delta(const sig3d_rel_attention_args *a) { return ((long)a->b * a->h * a->nq + 3) / 4 * 4; }
+long work_blocks(const sig3d_rel_attention_args *a) { return (long)a->b * sig3d_ceil_div(a->nq, NW * 32) * NW * 4; }
+long work_tops(const sig3d_rel_attention_args *a) {
+  return a->dtype == 2 ? (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * NW : 0;
+}
+long work_hist(const sig3d_rel_attention_args *a) {
+  return a->buckets.n > 0 ? (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * a->table_rows : 0;
+}
+
+template <typename T, int D> int launch_fwd(const Params &p, hipStream_t stream) {
+  static sig3d_once_per_device once;
+  const size_t lds = 4 * key_tile<T>() * Tile<T, D>::ROW + (2 * p.bk.reach + 1) * sizeof(float);
+  if (int e = allow_lds(rel_fwd_kernel<T, D, NW>, once)) return e;
+  rel_fwd_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, lds, stream>>>(p);
+  SIG3D_LAUNCH_CHECK("rel_fwd_kernel");
+  return 0;
+}
+
+template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream) {
+  static sig3d_once_per_device once_q, once_kv;
+  const int span = 2 * p.bk.reach + 1;
+  const size_t tiles = 4 * key_tile<T>() * Tile<T, D>::ROW;
+  if (int e = allow_lds(rel_bwd_dq_kernel<T, D, NW>, once_q)) return e;
+  if (int e = allow_lds(rel_bwd_dkv_kernel<T, D, NW>, once_kv)) return e;
+  rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, tiles + (NW + 1) * span * sizeof(float), stream>>>(p);
+  SIG3D_LAUNCH_CHECK("rel_bwd_dq_kernel");
+  rel_bwd_dkv_kernel<T, D, NW><<<p.b * p.hkv * p.ktiles, NW * 64, tiles + span * sizeof(float), stream>>>(p);
+  SIG3D_LAUNCH_CHECK("rel_bwd_dkv_kernel");
+  if (p.bk.n > 0) {
+    rel_bwd_table_kernel<T><<<dim3(p.h, sig3d_ceil_div(p.table_rows, 4)), 256, 0, stream>>>(
+        p.hist, p.b, p.h, p.qtiles, p.table_rows, reinterpret_cast<T *>(p.dtable));
+    SIG3D_LAUNCH_CHECK("rel_bwd_table_kernel");
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int sig3d_rel_attention_fwd(const sig3d_rel_attention_args *a, void *stream) {
+  if (int e = check("sig3d_rel_attention_fwd", a)) return e;
+  const Params p = params(a);
+  return by_type(a->dtype, a->d, [&](auto t, auto d) {
+    return launch_fwd<decltype(t), decltype(d)::value>(p, (hipStream_t)stream);
+  });
+}
+
+extern "C" long sig3d_rel_attention_bwd_work_floats(const sig3d_rel_attention_args *a) {
+  if (check("sig3d_rel_attention_bwd_work_floats", a)) return -1;
+  return work_delta(a) + work_blocks(a) + work_tops(a) + work_hist(a);
+}
+
+extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *stream) {
+  if (int e = check("sig3d_rel_attention_bwd", a)) return e;
+  const int e = a->dtype == 0 ? 4 : 2;
+  SIG3D_REQUIRE(a->out32 && a->lse && a->grad && a->dq && a->dk && a->dv && a->work, "missing array");
+  SIG3D_REQUIRE(aligned16(a->grad) && aligned16(a->dq) && aligned16(a->dk) && aligned16(a->dv) && aligned16(a->work),
+                "addresses must be 16-byte aligned");
+  SIG3D_REQUIRE(a->grad_b >= 0 && a->grad_n >= 0 && a->grad_h >= 0 && a->grad_b * e % 16 == 0 && a->grad_n * e % 16 == 0 &&
+                    a->grad_h * e % 16 == 0, "strides must be non-negative multiples of 16 bytes");
+  SIG3D_REQUIRE(a->buckets.n == 0 || a->dtable, "a bias needs dtable");
+  Params p = params(a);
+  p.delta = a->work;
+  p.blocks = reinterpret_cast<int4 *>(a->work + work_delta(a));
+  p.tops = reinterpret_cast<int *>(a->work + work_delta(a) + work_blocks(a));
+  p.hist = a->work + work_delta(a) + work_blocks(a) + work_tops(a);
+  return by_type(a->dtype, a->d, [&](auto t, auto d) {
+    return launch_bwd<decltype(t), decltype(d)::value>(p, (hipStream_t)stream);
+  });
+}
