@@ -22,6 +22,7 @@ namespace {
 using namespace lang;
 
 constexpr int WAVES = 4, KT = 32;
+constexpr float SLACK = 8.f;
 
 struct Side { const void *k, *v; const float *k_scale, *v_scale; int capacity; };
 struct DecodeParams {
@@ -32,7 +33,8 @@ struct DecodeParams {
   float *part;               // pieces: D + 2 floats a row and piece (output, max, sum)
   long q_b, q_n, q_h;
   int b, t, h, hkv, group, each;       // each: sequences of a shared prefix (0: nothing is shared)
-  int own_splits, shared_splits, own_tiles, shared_tiles, shared_items, bias_heads;
+  int own_splits, shared_splits;       // most pieces of a row's own and shared keys (see piece_rows)
+  int own_tiles, shared_tiles, shared_items, bias_heads;
   int joined;                // own items walk the shared rows too, no shared items
   int direct;                // one piece a row: the result is written here
   float scale;
@@ -50,37 +52,33 @@ template <typename T, int D, bool Q> struct Flight {
   uint2 vq[Q ? VN : 1];
   float vs[Q ? VN : 1];
 
-  __device__ __forceinline__ void load(const Side &s, long row0, int k0, int end, int lane) {
-    const int m = lane & 15, g = lane >> 4, last = end - 1;
+  // k, v, k_scale, v_scale: the tile's first row (uniform over the wave, so that a load is one scalar base and a 32-bit offset);
+  // n: rows of the tile that exist.  Loads of rows beyond them repeat the last one: scores are masked, put_v zeroes.
+  __device__ __forceinline__ void load(const char *kp, const char *vp, const float *k_scale, const float *v_scale, int n, int lane) {
+    constexpr int ROW = D * (Q ? 1 : (int)sizeof(T));
+    const int m = lane & 15, g = lane >> 4, last = n - 1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const long row = row0 + min(k0 + 8 * (m >> 2) + 4 * t + (m & 3), last);      // beyond the end: any row, masked later
+      const unsigned row = min(8 * (m >> 2) + 4 * t + (m & 3), last);
       if constexpr (Q) {
-        ks[t] = s.k_scale[row];
+        ks[t] = k_scale[row];
 #pragma unroll
         for (int f = 0; f < KS; ++f)       // lane group g holds D / 4 consecutive values: 16 bytes a load, and Q likewise
-          kq[t][f] = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(s.k) + row * D + g * (D / 4) + 8 * f);
+          kq[t][f] = *reinterpret_cast<const uint2 *>(kp + (row * ROW + g * (D / 4) + 8 * f));
       } else {
 #pragma unroll
         for (int f = 0; f < KS; ++f)
-          k[t][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(s.k) + row * D + 32 * f + 8 * g);
+          k[t][f] = *reinterpret_cast<const frag_t<T> *>(kp + (row * ROW + (32 * f + 8 * g) * (unsigned)sizeof(T)));
       }
     }
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
-      const int c = lane + 64 * i, r = c / (D / 8), o = c - r * (D / 8);
-      const bool ok = k0 + r < end;
-      const long row = row0 + k0 + r;
+      const unsigned c = lane + 64 * i, r = c / (D / 8), o = c - r * (D / 8), row = min((int)r, last);
       if constexpr (Q) {
-        vq[i] = make_uint2(0, 0);
-        vs[i] = 1.f;
-        if (ok) {
-          vq[i] = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(s.v) + row * D + 8 * o);
-          vs[i] = s.v_scale[row];
-        }
+        vq[i] = *reinterpret_cast<const uint2 *>(vp + (row * ROW + 8 * o));
+        vs[i] = v_scale[row];
       } else {
-        v[i] = frag_t<T>{};
-        if (ok) v[i] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(s.v) + row * D + 8 * o);
+        v[i] = *reinterpret_cast<const frag_t<T> *>(vp + (row * ROW + 8 * o * (unsigned)sizeof(T)));
       }
     }
   }
@@ -88,7 +86,7 @@ template <typename T, int D, bool Q> struct Flight {
     if constexpr (Q) return from_e4m3<T>(kq[t][f], ks[t]);
     else return k[t][f];
   }
-  __device__ __forceinline__ void put_v(char *tile, int lane) const {
+  __device__ __forceinline__ void put_v(char *tile, int n, int lane) const {
     typedef Tile<T, D> TL;
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
@@ -96,6 +94,7 @@ template <typename T, int D, bool Q> struct Flight {
       frag_t<T> x;
       if constexpr (Q) x = from_e4m3<T>(vq[i], vs[i]);
       else x = v[i];
+      if (n < KT && r >= n) x = frag_t<T>{};
       if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<frag_t<T> *>(tile + TL::at(r, o)) = x;
       } else {
@@ -109,24 +108,38 @@ template <typename T, int D, bool Q> struct Flight {
 // which element of a head fragment f of lane group g starts at (see Flight::load)
 template <int D, bool Q> __device__ __forceinline__ int element(int f, int g) { return Q ? g * (D / 4) + 8 * f : 32 * f + 8 * g; }
 
-__device__ __forceinline__ float max_groups(float x) {      // over the four 16-lane groups
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return max_halves(x);
+// over the four 16-lane groups
+__device__ __forceinline__ void both_groups(float x, float &lo, float &hi) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  const unsigned a = s[0], b = s[1];
+  lo = __builtin_bit_cast(float, a);
+  hi = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float max_groups(float x) {
+  float lo, hi;
+  both_groups(x, lo, hi);
+  return max_halves(fmaxf(lo, hi));
 }
 __device__ __forceinline__ float sum_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return sum_halves(x);
+  float lo, hi;
+  both_groups(x, lo, hi);
+  return sum_halves(lo + hi);
 }
 
-// What one row of queries is.
-struct RowInfo { int head, j, seq, pos, end; };    // pos: own row of the query (below 0: no query); end = pos + 1 own rows seen
+// The tiles of a sequence are cut into at most `most` pieces of equal length, of at least LEAST tiles (two a wave: below that a
+// workgroup is all start and join).  Short sequences of a ragged batch have few pieces, and the workgroups of the others leave
+// at once; long ones do not get longer pieces than they must.
+constexpr int LEAST = 2 * WAVES;
+__device__ __forceinline__ int piece_tiles(int tiles, int most) { return max(LEAST, (tiles + most - 1) / most); }
+__device__ __forceinline__ int clamp_rows(int n, int capacity) { return min(max(n, 0), capacity); }
+__device__ __forceinline__ int tiles_of(int rows) { return (rows + KT - 1) / KT; }
 
 template <typename T, int D, bool Q, int NB>
 __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool shared, char *lds) {
   typedef Tile<T, D> TL;
   typedef Flight<T, D, Q> FL;
   constexpr int KS = FL::KS, TB = KT * TL::ROW, DT = D / 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
   char *vt = lds + wave * TB;
   float *bias = reinterpret_cast<float *>(lds + WAVES * TB);
   float *stat = bias + p.bias_heads * (p.bk.reach + 1);                    // [2][WAVES][16]
@@ -141,29 +154,32 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   const int per = p.group * p.t, rows = shared ? p.each * per : per;
   const int r0 = rt * 16 * NB;
 
-  RowInfo info[NB];
+  const int shared_len = p.each && (shared || p.joined)
+                             ? clamp_rows(p.shared_lengths[shared ? unit : unit / p.each], p.shared.capacity) : 0;
+  const int own_len = shared ? 0 : clamp_rows(p.lengths[unit], p.own.capacity);
+  // the piece, in tiles: those of the shared rows, then those of the own rows
+  const int far_tiles = tiles_of(shared_len), all_tiles = far_tiles + tiles_of(own_len);
+  const int share = piece_tiles(all_tiles, splits), from = piece * share, to = min(from + share, all_tiles);
+  if (piece > 0 && from >= all_tiles) return;
+
+  int pos[NB], qhead[NB];                    // own row of the query (below 0: no query); its head
   frag_t<T> qf[NB][KS];
-  const int shared_len = p.each ? (shared || p.joined ? min(max(p.shared_lengths[shared ? unit : unit / p.each], 0), p.shared.capacity) : 0) : 0;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const int r = r0 + 16 * n + col, in = r % per;
-    info[n].seq = shared ? unit * p.each + r / per : unit;
-    info[n].head = kvh * p.group + in / p.t;
-    info[n].j = in % p.t;
-    info[n].pos = -1;
+    const int r = r0 + 16 * n + col, in = r % per, seq = shared ? unit * p.each + r / per : unit, j = in % p.t;
+    qhead[n] = kvh * p.group + in / p.t;
+    pos[n] = -1;
     if (r < rows) {
-      const int len = min(max(p.lengths[info[n].seq], 0), p.own.capacity);
-      const int count = p.counts ? min(max(p.counts[info[n].seq], 0), p.t) : p.t;
-      if (info[n].j < count) info[n].pos = max(len - count + info[n].j, -1);
+      const int len = clamp_rows(p.lengths[seq], p.own.capacity);
+      const int count = p.counts ? clamp_rows(p.counts[seq], p.t) : p.t;
+      if (j < count) pos[n] = max(len - count + j, -1);
     }
-    info[n].end = info[n].pos + 1;
-    const bool ok = info[n].pos >= 0;
 #pragma unroll
     for (int f = 0; f < KS; ++f) {
       qf[n][f] = frag_t<T>{};
-      if (ok)
-        qf[n][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.q) + info[n].seq * p.q_b +
-                                                       (long)info[n].j * p.q_n + info[n].head * p.q_h + element<D, Q>(f, g));
+      if (pos[n] >= 0)
+        qf[n][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.q) + seq * p.q_b + (long)j * p.q_n +
+                                                       qhead[n] * p.q_h + element<D, Q>(f, g));
     }
   }
   const bool biased = p.bk.n > 0;
@@ -177,19 +193,17 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
     }
     __syncthreads();
   }
-  const float *mine[NB];
+  int mine[NB];                              // where the head's biases start
   float farthest[NB];
-  int longest = 0, lowest = INT_MAX;         // own rows seen by any row here; lowest position of a query
+  int lowest = INT_MAX;                      // position of the first query here
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    int hh = info[n].head - head0;
+    int hh = qhead[n] - head0;
     if (hh < 0) hh += p.group;
-    mine[n] = bias + min(hh, max(p.bias_heads - 1, 0)) * (reach + 1);
-    farthest[n] = biased ? mine[n][reach] : 0.f;
-    longest = max(longest, info[n].end);
-    if (info[n].pos >= 0) lowest = min(lowest, info[n].pos);
+    mine[n] = min(hh, max(p.bias_heads - 1, 0)) * (reach + 1);
+    farthest[n] = biased ? bias[mine[n] + reach] : 0.f;
+    if (pos[n] >= 0) lowest = min(lowest, pos[n]);
   }
-  longest = wave_max_i32(longest);
   lowest = wave_min_i32(lowest);
 
   f32x4 o[NB][DT] = {};
@@ -198,21 +212,23 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   for (int n = 0; n < NB; ++n) { m[n] = -INFINITY; l[n] = 0.f; }
   const float scale2 = p.scale * LOG2E;
 
-  // the piece: tiles of the shared rows, then of the own rows
-  const int own_len = shared ? 0 : longest, far_len = longest > 0 ? shared_len : 0;
-  const int far_tiles = (far_len + KT - 1) / KT, all_tiles = far_tiles + (own_len + KT - 1) / KT;
-  const int share = (all_tiles + splits - 1) / splits, from = piece * share, to = min(from + share, all_tiles);
   const long far_row = ((long)(shared ? unit : (p.each ? unit / p.each : 0)) * p.hkv + kvh) * p.shared.capacity;
   const long own_row = ((long)unit * p.hkv + kvh) * p.own.capacity;
   FL fl;
   auto fetch = [&](int tile) {
     const bool far = tile < far_tiles;
-    fl.load(far ? p.shared : p.own, far ? far_row : own_row, (far ? tile : tile - far_tiles) * KT, far ? far_len : own_len, lane);
+    const int k0 = (far ? tile : tile - far_tiles) * KT;
+    const long row = (far ? far_row : own_row) + k0;
+    constexpr int ROW = D * (Q ? 1 : (int)sizeof(T));
+    const void *kp = far ? p.shared.k : p.own.k, *vp = far ? p.shared.v : p.own.v;
+    const float *ksp = far ? p.shared.k_scale : p.own.k_scale, *vsp = far ? p.shared.v_scale : p.own.v_scale;
+    fl.load(reinterpret_cast<const char *>(kp) + row * ROW, reinterpret_cast<const char *>(vp) + row * ROW, ksp + row, vsp + row,
+            min((far ? shared_len : own_len) - k0, KT), lane);
   };
   if (from + wave < to) fetch(from + wave);
   for (int tile = from + wave; tile < to; tile += WAVES) {
     const bool far = tile < far_tiles;
-    const int k0 = (far ? tile : tile - far_tiles) * KT, end = far ? far_len : own_len;
+    const int k0 = (far ? tile : tile - far_tiles) * KT, end = far ? shared_len : own_len;
     // distance of a query at own row pos from key 0 of the tile: shared rows stand before the own ones
     const int ahead = far ? shared_len - k0 : -k0;
     f32x4 s[NB][2] = {};
@@ -224,7 +240,7 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[n][t] = mma16(kf, qf[n][f], s[n][t]);
       }
-    fl.put_v(vt, lane);
+    fl.put_v(vt, min(end - k0, KT), lane);
     if (tile + WAVES < to) fetch(tile + WAVES);
     const bool near = biased && lowest + ahead - (KT - 1) < reach;
     const bool cut = k0 + KT > end || (!far && k0 + KT > lowest + 1);
@@ -236,10 +252,10 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
       for (int j = 0; j < 8; ++j) x[j] = __builtin_fmaf(s[n][j >> 2][j & 3], scale2, near ? 0.f : farthest[n]);
       if (near) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += mine[n][min(max(info[n].pos + ahead - 8 * g - j, 0), reach)];
+        for (int j = 0; j < 8; ++j) x[j] += bias[mine[n] + min(max(pos[n] + ahead - 8 * g - j, 0), reach)];
       }
       if (cut) {
-        const int seen = far ? end : min(end, info[n].end);
+        const int seen = far ? end : min(end, pos[n] + 1);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (k0 + 8 * g + j >= seen) x[j] = -INFINITY;
@@ -247,9 +263,8 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
       float top = x[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-      top = max_groups(top);
-      if (__any(top > m[n])) {
-        const float now = fmaxf(m[n], top);
+      if (__any(top > m[n] + SLACK)) {       // exponentials up to 2^SLACK are as good as up to 1: the maximum seldom moves
+        const float now = fmaxf(m[n], max_groups(top));
         const float keep = now == -INFINITY ? 1.f : exp2_(m[n] - now);
         m[n] = now;
         l[n] *= keep;
@@ -281,7 +296,7 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   float *mine_o = reinterpret_cast<float *>(lds);                           // [WAVES][16][D]; the V tiles are done with
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const bool live = info[n].pos >= 0;                                     // what is no query has seen the shared rows for nothing
+    const bool live = pos[n] >= 0;                                          // what is no query has seen the shared rows for nothing
     const float sum = live ? sum_groups(l[n]) : 0.f;
     if (!live) m[n] = -INFINITY;
     __syncthreads();
@@ -338,46 +353,86 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   }
 }
 
+// Two waves a SIMD: a wave's loads hide behind another one's arithmetic (f32 keeps its registers: 512 a lane).
 template <typename T, int D, bool Q, int NB>
-__global__ __launch_bounds__(WAVES * 64) void decode_kernel(const DecodeParams p) {
+__global__ __launch_bounds__(WAVES * 64, sizeof(T) == 2 ? 2 : 1) void decode_kernel(const DecodeParams p) {
   extern __shared__ __align__(16) char lds[];
   if ((int)blockIdx.x < p.shared_items) walk<T, D, Q, NB>(p, blockIdx.x, true, lds);
   else walk<T, D, Q, 1>(p, blockIdx.x - p.shared_items, false, lds);
 }
 
-// Joins the pieces of a row, shared ones first: D / 4 lanes a row.
+// Joins the pieces of a row, shared ones first.  A wave owns a row: lane i weighs piece i (64 at a time), then groups of D / 4
+// lanes add every (64 / (D / 4))-th piece and the groups are added in their order.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
-  constexpr int PER = D / 4, ROWS = 256 / PER;
-  const int per = p.group * p.t, e = threadIdx.x % PER;
-  const long row = (long)blockIdx.x * ROWS + threadIdx.x / PER;              // (sequence, key head, head of the group, token)
-  if (threadIdx.x / PER >= ROWS || row >= (long)p.b * p.hkv * per) return;
-  const int in = (int)(row % per);
-  const int kvh = (int)(row / per % p.hkv), seq = (int)(row / per / p.hkv);
-  const float *own = p.part + ((long)p.shared_splits * p.b * p.hkv * per + row * p.own_splits) * (D + 4);
+  constexpr int PER = D / 4, GROUPS = 64 / PER, STEP = D + 4;
+  __shared__ float weight[4][64];
+  __shared__ __align__(16) float partial[4][GROUPS][D];
+  const int per = p.group * p.t, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.x * 4 + wave;                                     // (sequence, key head, head of the group, token)
+  if (row >= p.b * p.hkv * per) return;
+  const int in = row % per, kvh = row / per % p.hkv, seq = row / per / p.hkv;
+  const int far_tiles = p.each ? tiles_of(clamp_rows(p.shared_lengths[seq / p.each], p.shared.capacity)) : 0;
+  const int own_tiles = tiles_of(clamp_rows(p.lengths[seq], p.own.capacity)) + (p.joined ? far_tiles : 0);
+  const int own_piece = piece_tiles(own_tiles, p.own_splits), own_n = max(1, (own_tiles + own_piece - 1) / own_piece);
+  const float *own = p.part + ((long)p.shared_splits * p.b * p.hkv * per + (long)row * p.own_splits) * STEP;
+  int far_n = 0;
   const float *far = nullptr;
-  if (p.shared_splits)
-    far = p.part + ((((long)(seq / p.each) * p.hkv + kvh) * p.each + seq % p.each) * per + in) * p.shared_splits * (D + 4);
-  float top = -INFINITY;
-  for (int s = 0; s < p.shared_splits; ++s) top = fmaxf(top, far[s * (D + 4) + D]);
-  for (int s = 0; s < p.own_splits; ++s) top = fmaxf(top, own[s * (D + 4) + D]);
-  const float base = top == -INFINITY ? 0.f : top;
+  if (p.shared_splits) {
+    const int piece = piece_tiles(far_tiles, p.shared_splits);
+    far_n = max(1, (far_tiles + piece - 1) / piece);
+    far = p.part + ((((long)(seq / p.each) * p.hkv + kvh) * p.each + seq % p.each) * per + in) * p.shared_splits * STEP;
+  }
+  const int n = far_n + own_n, grp = lane / PER, e = lane % PER;
+  float top = -INFINITY, sum = 0.f;
   f32x4 x = {};
-  float sum = 0.f;
-  auto add = [&](const float *piece) {
-    const float keep = exp2_(piece[D] - base);
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(piece + 4 * e);
-    sum += piece[D + 1] * keep;
+  for (int first = 0; first < n; first += 64) {
+    const int i = first + lane, last = min(n - first, 64);
+    float m = -INFINITY, l = 0.f;
+    if (i < n) {
+      const float *piece = i < far_n ? far + (long)i * STEP : own + (long)(i - far_n) * STEP;
+      m = piece[D];
+      l = piece[D + 1];
+    }
+    float now = m;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(y[q], keep, x[q]);
-  };
-  for (int s = 0; s < p.shared_splits; ++s) add(far + s * (D + 4));
-  for (int s = 0; s < p.own_splits; ++s) add(own + s * (D + 4));
-  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    for (int s = 1; s < 64; s <<= 1) now = fmaxf(now, __shfl_xor(now, s));
+    now = fmaxf(now, top);
+    const float base = now == -INFINITY ? 0.f : now, keep = exp2_(top - base), w = exp2_(m - base);
+    weight[wave][lane] = w;
+    sum = sum * keep + wave_allreduce_sum_f32(l * w);
+    top = now;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) x[q] *= inv;
-  const long at = (((long)seq * p.t + in % p.t) * p.h + kvh * p.group + in / p.t) * D + 4 * e;
-  *reinterpret_cast<vec4_t<T> *>(reinterpret_cast<T *>(p.out) + at) = to_vec4<T>(x);
+    for (int q = 0; q < 4; ++q) x[q] *= keep;
+    __builtin_amdgcn_wave_barrier();
+    if (grp < GROUPS) {
+#pragma unroll 4
+      for (int j = grp; j < last; j += GROUPS) {
+        const int k = first + j;
+        const float *piece = k < far_n ? far + (long)k * STEP : own + (long)(k - far_n) * STEP;
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(piece + 4 * e);
+        const float wj = weight[wave][j];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(y[q], wj, x[q]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (grp < GROUPS) *reinterpret_cast<f32x4 *>(&partial[wave][grp][4 * e]) = x;
+  __builtin_amdgcn_wave_barrier();
+  if (lane < PER) {
+#pragma unroll
+    for (int s = 1; s < GROUPS; ++s) {
+      const f32x4 y = *reinterpret_cast<const f32x4 *>(&partial[wave][s][4 * lane]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] += y[q];
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] *= inv;
+    const long at = (((long)seq * p.t + in % p.t) * p.h + kvh * p.group + in / p.t) * D + 4 * lane;
+    *reinterpret_cast<vec4_t<T> *>(reinterpret_cast<T *>(p.out) + at) = to_vec4<T>(x);
+  }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
@@ -396,6 +451,9 @@ int check(const char *where, const sig3d_decode_attention_args *a) {
   return check_buckets(where, a->buckets, a->table, a->table_rows);
 }
 
+// Blocks of 16 query rows a workgroup takes over shared keys: what two waves a SIMD leave registers for.
+constexpr int blocks_of_rows(int dtype, int d) { return dtype != 0 && d == 64 ? 4 : 2; }
+
 Plan plan(const sig3d_decode_attention_args *a) {
   Plan s = {};
   const int group = a->h / a->hkv, per = group * a->t, each = a->groups ? a->b / a->groups : 0;
@@ -406,15 +464,14 @@ Plan plan(const sig3d_decode_attention_args *a) {
   // where they are short.
   s.joined = each > 0 && (each == 1 || a->shared_capacity <= 256);
   s.nb = 1;
-  const int piece = 8 * KT;             // two tiles a wave: a piece below that is all start and join
   const int own_rows = a->capacity + (s.joined ? a->shared_capacity : 0);
-  s.own_splits = (int)std::min<long>(std::max<long>(1, 1024 / base), sig3d_ceil_div(own_rows, piece));
+  s.own_splits = (int)std::min<long>(std::max<long>(1, 4096 / base), sig3d_ceil_div(own_rows, LEAST * KT));
   if (each > 0 && !s.joined) {
     const long rows = (long)each * per;
-    s.nb = rows > 16 ? 4 : 1;
+    s.nb = rows > 16 ? blocks_of_rows(a->dtype, a->d) : 1;
     s.shared_tiles = sig3d_ceil_div(rows, 16 * s.nb);
     const long far = (long)a->groups * a->hkv * s.shared_tiles;
-    s.shared_splits = (int)std::min<long>(std::max<long>(1, 1024 / far), sig3d_ceil_div(a->shared_capacity, piece));
+    s.shared_splits = (int)std::min<long>(std::max<long>(1, 2048 / far), sig3d_ceil_div(a->shared_capacity, LEAST * KT));
     s.shared_items = (int)(far * s.shared_splits);
   }
   s.own_items = (int)(base * s.own_splits);
@@ -431,8 +488,7 @@ template <typename T, int D, bool Q, int NB> int launch(const DecodeParams &p, c
   decode_kernel<T, D, Q, NB><<<s.shared_items + s.own_items, WAVES * 64, s.lds, stream>>>(p);
   SIG3D_LAUNCH_CHECK("decode_kernel");
   if (!p.direct) {
-    const long rows = (long)p.b * p.hkv * p.group * p.t;
-    decode_join_kernel<T, D><<<sig3d_ceil_div(rows, 256 / (D / 4)), 256, 0, stream>>>(p);
+    decode_join_kernel<T, D><<<sig3d_ceil_div((long)p.b * p.h * p.t, 4), 256, 0, stream>>>(p);
     SIG3D_LAUNCH_CHECK("decode_join_kernel");
   }
   return 0;
@@ -477,7 +533,8 @@ extern "C" int sig3d_decode_attention(const sig3d_decode_attention_args *a, void
   return by_type(a->dtype, a->d, [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
-    if (s.nb == 4) return quantized ? launch<T, D, true, 4>(p, s, (hipStream_t)stream) : launch<T, D, false, 4>(p, s, (hipStream_t)stream);
+    constexpr int NB = blocks_of_rows(sizeof(T) == 4 ? 0 : 1, D);
+    if (s.nb == NB) return quantized ? launch<T, D, true, NB>(p, s, (hipStream_t)stream) : launch<T, D, false, NB>(p, s, (hipStream_t)stream);
     return quantized ? launch<T, D, true, 1>(p, s, (hipStream_t)stream) : launch<T, D, false, 1>(p, s, (hipStream_t)stream);
   });
 }

@@ -148,7 +148,7 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
   float *bias = reinterpret_cast<float *>(lds + 4 * TB);
   __shared__ int ends[2][NW];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;      // causal: the long rows first
   const int b = bh / p.h, head = bh - b * p.h;
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
   float *sums = bias + span;                              // [NW][span]
   __shared__ int ends[2][NW];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;
   const int b = bh / p.h, head = bh - b * p.h;
@@ -509,7 +509,7 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dkv_kernel(const Params p) {
   float *bias = reinterpret_cast<float *>(lds + 4 * TB);
   const int reach = p.bk.reach;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int bh = id / p.ktiles, kt0 = id % p.ktiles;
   const int b = bh / p.hkv, kvh = bh - b * p.hkv;
