@@ -34,7 +34,7 @@ struct DecodeParams {
   long q_b, q_n, q_h;
   int b, t, h, hkv, group, each;       // each: sequences of a shared prefix (0: nothing is shared)
   int own_splits, shared_splits;       // most pieces of a row's own and shared keys (see piece_rows)
-  int own_tiles, shared_tiles, shared_items, bias_heads;
+  int own_tiles, shared_tiles, own_items, shared_items, own_bias_heads, shared_bias_heads;
   int joined;                // own items walk the shared rows too, no shared items
   int direct;                // one piece a row: the result is written here
   float scale;
@@ -44,12 +44,13 @@ struct DecodeParams {
 // One 32-key tile of one side on its way from memory.
 template <typename T, int D, bool Q> struct Flight {
   static constexpr int KS = D / 32;                         // reduction steps of a score
-  static constexpr int VN = D / 16;                         // 8-element pieces of V a lane carries
+  static constexpr int VE = Q ? 16 : 8;                     // elements of a piece of V: 16 bytes in 8 or 16 bits
+  static constexpr int VN = KT * D / VE / 64;               // pieces of V a lane carries
   frag_t<T> k[2][Q ? 1 : KS];
   uint2 kq[2][Q ? KS : 1];
   float ks[2];
   frag_t<T> v[Q ? 1 : VN];
-  uint2 vq[Q ? VN : 1];
+  uint4 vq[Q ? VN : 1];
   float vs[Q ? VN : 1];
 
   // k, v, k_scale, v_scale: the tile's first row (uniform over the wave, so that a load is one scalar base and a 32-bit offset);
@@ -73,12 +74,12 @@ template <typename T, int D, bool Q> struct Flight {
     }
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
-      const unsigned c = lane + 64 * i, r = c / (D / 8), o = c - r * (D / 8), row = min((int)r, last);
+      const unsigned c = lane + 64 * i, r = c / (D / VE), o = c - r * (D / VE), row = min((int)r, last);
       if constexpr (Q) {
-        vq[i] = *reinterpret_cast<const uint2 *>(vp + (row * ROW + 8 * o));
+        vq[i] = *reinterpret_cast<const uint4 *>(vp + (row * ROW + VE * o));
         vs[i] = v_scale[row];
       } else {
-        v[i] = *reinterpret_cast<const frag_t<T> *>(vp + (row * ROW + 8 * o * (unsigned)sizeof(T)));
+        v[i] = *reinterpret_cast<const frag_t<T> *>(vp + (row * ROW + VE * o * (unsigned)sizeof(T)));
       }
     }
   }
@@ -87,20 +88,25 @@ template <typename T, int D, bool Q> struct Flight {
     else return k[t][f];
   }
   __device__ __forceinline__ void put_v(char *tile, int n, int lane) const {
-    typedef Tile<T, D> TL;
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
-      const int c = lane + 64 * i, r = c / (D / 8), o = c - r * (D / 8);
-      frag_t<T> x;
-      if constexpr (Q) x = from_e4m3<T>(vq[i], vs[i]);
-      else x = v[i];
-      if (n < KT && r >= n) x = frag_t<T>{};
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<frag_t<T> *>(tile + TL::at(r, o)) = x;
+      const int c = lane + 64 * i, r = c / (D / VE), o = c - r * (D / VE);
+      const bool none = n < KT && r >= n;
+      if constexpr (Q) {
+        put_piece(tile, r, 2 * o, none ? frag_t<T>{} : from_e4m3<T>(make_uint2(vq[i].x, vq[i].y), vs[i]));
+        put_piece(tile, r, 2 * o + 1, none ? frag_t<T>{} : from_e4m3<T>(make_uint2(vq[i].z, vq[i].w), vs[i]));
       } else {
-        *reinterpret_cast<f32x4 *>(tile + TL::at(r, 2 * o)) = __builtin_shufflevector(x, x, 0, 1, 2, 3);
-        *reinterpret_cast<f32x4 *>(tile + TL::at(r, 2 * o + 1)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+        put_piece(tile, r, o, none ? frag_t<T>{} : v[i]);
       }
+    }
+  }
+  static __device__ __forceinline__ void put_piece(char *tile, int r, int o, frag_t<T> x) {
+    typedef Tile<T, D> TL;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<frag_t<T> *>(tile + TL::at(r, o)) = x;
+    } else {
+      *reinterpret_cast<f32x4 *>(tile + TL::at(r, 2 * o)) = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+      *reinterpret_cast<f32x4 *>(tile + TL::at(r, 2 * o + 1)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
     }
   }
 };
@@ -129,20 +135,28 @@ __device__ __forceinline__ float sum_groups(float x) {
 // The tiles of a sequence are cut into at most `most` pieces of equal length, of at least LEAST tiles (two a wave: below that a
 // workgroup is all start and join).  Short sequences of a ragged batch have few pieces, and the workgroups of the others leave
 // at once; long ones do not get longer pieces than they must.
-constexpr int LEAST = 2 * WAVES;
+constexpr int LEAST = 4 * WAVES;
 __device__ __forceinline__ int piece_tiles(int tiles, int most) { return max(LEAST, (tiles + most - 1) / most); }
 __device__ __forceinline__ int clamp_rows(int n, int capacity) { return min(max(n, 0), capacity); }
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + KT - 1) / KT; }
 
-template <typename T, int D, bool Q, int NB>
+// LDS tiles of V a wave has
+template <typename T, int D> constexpr int TILES = D == 64 && sizeof(T) == 2 ? 2 : 1;
+
+// One item: 16 NB query rows over one piece of their keys, by WV = 4 waves of a workgroup (a wave every fourth tile, joined
+// through LDS) or by one wave alone.
+template <typename T, int D, bool Q, int NB, int WV>
 __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool shared, char *lds) {
   typedef Tile<T, D> TL;
   typedef Flight<T, D, Q> FL;
   constexpr int KS = FL::KS, TB = KT * TL::ROW, DT = D / 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
-  char *vt = lds + wave * TB;
-  float *bias = reinterpret_cast<float *>(lds + WAVES * TB);
-  float *stat = bias + p.bias_heads * (p.bk.reach + 1);                    // [2][WAVES][16]
+  // tiles a step: a lone wave has nobody to hide its latencies behind but its own second tile
+  constexpr int NT = WV == 1 ? TILES<T, D> : 1;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int wave = WV == 1 ? 0 : wv, tid = WV == 1 ? lane : threadIdx.x;   // among those that share the item
+  char *vt = lds + wv * TILES<T, D> * TB;
+  const int heads = shared ? p.shared_bias_heads : p.own_bias_heads, reach = p.bk.reach;
+  float *bias = reinterpret_cast<float *>(lds + WAVES * TILES<T, D> * TB) + (WV == 1 ? wv * heads * (reach + 1) : 0);
 
   // item -> (sequence or group, key head, block of rows, piece)
   const int splits = shared ? p.shared_splits : p.own_splits, tiles = shared ? p.shared_tiles : p.own_tiles;
@@ -154,6 +168,20 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   const int per = p.group * p.t, rows = shared ? p.each * per : per;
   const int r0 = rt * 16 * NB;
 
+  // log2(e) * bias of the heads of these rows by distance behind the query.  These loads go out before those of keys and
+  // queries: loads return in order, and these are two in a row (bucket, entry).
+  const bool biased = p.bk.n > 0;
+  const int in0 = shared ? r0 % per : r0, gi0 = p.t == 1 ? in0 : in0 / p.t, biases = biased ? heads * (reach + 1) : 0;
+  const T *table = reinterpret_cast<const T *>(p.table);
+  auto bias_at = [&](int i) {
+    int hh = heads == 1 ? 0 : i / (reach + 1);
+    const int a = i - hh * (reach + 1);
+    hh += gi0;
+    return (float)table[(long)bucket_of(p.bk, -a) * p.h + kvh * p.group + (hh >= p.group ? hh - p.group : hh)] * LOG2E;
+  };
+  float first_bias = 0.f;
+  if (tid < biases) first_bias = bias_at(tid);
+
   const int shared_len = p.each && (shared || p.joined)
                              ? clamp_rows(p.shared_lengths[shared ? unit : unit / p.each], p.shared.capacity) : 0;
   const int own_len = shared ? 0 : clamp_rows(p.lengths[unit], p.own.capacity);
@@ -162,15 +190,33 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   const int share = piece_tiles(all_tiles, splits), from = piece * share, to = min(from + share, all_tiles);
   if (piece > 0 && from >= all_tiles) return;
 
-  int pos[NB], qhead[NB];                    // own row of the query (below 0: no query); its head
+  const long far_row = ((long)(shared ? unit : (p.each ? unit / p.each : 0)) * p.hkv + kvh) * p.shared.capacity;
+  const long own_row = ((long)unit * p.hkv + kvh) * p.own.capacity;
+  FL fl[NT];
+  auto fetch = [&](FL &f, int tile) {
+    const bool far = tile < far_tiles;
+    const int k0 = (far ? tile : tile - far_tiles) * KT;
+    const long row = (far ? far_row : own_row) + k0;
+    constexpr int ROW = D * (Q ? 1 : (int)sizeof(T));
+    const void *kp = far ? p.shared.k : p.own.k, *vp = far ? p.shared.v : p.own.v;
+    const float *ksp = far ? p.shared.k_scale : p.own.k_scale, *vsp = far ? p.shared.v_scale : p.own.v_scale;
+    f.load(reinterpret_cast<const char *>(kp) + row * ROW, reinterpret_cast<const char *>(vp) + row * ROW, ksp + row, vsp + row,
+           min((far ? shared_len : own_len) - k0, KT), lane);
+  };
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+    if (from + wave + u * WV < to) fetch(fl[u], from + wave + u * WV);
+
+  int pos[NB], qhead[NB];                    // own row of the query (below 0: no query); its head in the group
   frag_t<T> qf[NB][KS];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const int r = r0 + 16 * n + col, in = r % per, seq = shared ? unit * p.each + r / per : unit, j = in % p.t;
-    qhead[n] = kvh * p.group + in / p.t;
+    const int r = r0 + 16 * n + col, sub = shared ? r / per : 0, in = r - sub * per, seq = shared ? unit * p.each + sub : unit;
+    qhead[n] = p.t == 1 ? in : in / p.t;
+    const int j = in - qhead[n] * p.t;
     pos[n] = -1;
     if (r < rows) {
-      const int len = clamp_rows(p.lengths[seq], p.own.capacity);
+      const int len = shared ? clamp_rows(p.lengths[seq], p.own.capacity) : own_len;
       const int count = p.counts ? clamp_rows(p.counts[seq], p.t) : p.t;
       if (j < count) pos[n] = max(len - count + j, -1);
     }
@@ -179,28 +225,23 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
       qf[n][f] = frag_t<T>{};
       if (pos[n] >= 0)
         qf[n][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.q) + seq * p.q_b + (long)j * p.q_n +
-                                                       qhead[n] * p.q_h + element<D, Q>(f, g));
+                                                       (kvh * p.group + qhead[n]) * p.q_h + element<D, Q>(f, g));
     }
   }
-  const bool biased = p.bk.n > 0;
-  const int head0 = kvh * p.group + (r0 % per) / p.t, reach = p.bk.reach;
-  const T *table = reinterpret_cast<const T *>(p.table);
-  if (biased) {        // log2(e) * bias of the heads of these rows by distance behind the query
-    for (int i = tid; i < p.bias_heads * (reach + 1); i += WAVES * 64) {
-      const int hh = i / (reach + 1), a = i - hh * (reach + 1);
-      const int head = kvh * p.group + (head0 - kvh * p.group + hh) % p.group;
-      bias[i] = (float)table[(long)bucket_of(p.bk, -a) * p.h + head] * LOG2E;
-    }
-    __syncthreads();
+  if (biased) {
+    if (tid < biases) bias[tid] = first_bias;
+    for (int i = tid + WV * 64; i < biases; i += WV * 64) bias[i] = bias_at(i);
+    if constexpr (WV == 1) __builtin_amdgcn_wave_barrier();
+    else __syncthreads();
   }
   int mine[NB];                              // where the head's biases start
   float farthest[NB];
   int lowest = INT_MAX;                      // position of the first query here
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    int hh = qhead[n] - head0;
+    int hh = qhead[n] - gi0;
     if (hh < 0) hh += p.group;
-    mine[n] = min(hh, max(p.bias_heads - 1, 0)) * (reach + 1);
+    mine[n] = min(hh, max(heads - 1, 0)) * (reach + 1);
     farthest[n] = biased ? bias[mine[n] + reach] : 0.f;
     if (pos[n] >= 0) lowest = min(lowest, pos[n]);
   }
@@ -212,57 +253,51 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   for (int n = 0; n < NB; ++n) { m[n] = -INFINITY; l[n] = 0.f; }
   const float scale2 = p.scale * LOG2E;
 
-  const long far_row = ((long)(shared ? unit : (p.each ? unit / p.each : 0)) * p.hkv + kvh) * p.shared.capacity;
-  const long own_row = ((long)unit * p.hkv + kvh) * p.own.capacity;
-  FL fl;
-  auto fetch = [&](int tile) {
-    const bool far = tile < far_tiles;
-    const int k0 = (far ? tile : tile - far_tiles) * KT;
-    const long row = (far ? far_row : own_row) + k0;
-    constexpr int ROW = D * (Q ? 1 : (int)sizeof(T));
-    const void *kp = far ? p.shared.k : p.own.k, *vp = far ? p.shared.v : p.own.v;
-    const float *ksp = far ? p.shared.k_scale : p.own.k_scale, *vsp = far ? p.shared.v_scale : p.own.v_scale;
-    fl.load(reinterpret_cast<const char *>(kp) + row * ROW, reinterpret_cast<const char *>(vp) + row * ROW, ksp + row, vsp + row,
-            min((far ? shared_len : own_len) - k0, KT), lane);
-  };
-  if (from + wave < to) fetch(from + wave);
-  for (int tile = from + wave; tile < to; tile += WAVES) {
-    const bool far = tile < far_tiles;
-    const int k0 = (far ? tile : tile - far_tiles) * KT, end = far ? shared_len : own_len;
-    // distance of a query at own row pos from key 0 of the tile: shared rows stand before the own ones
-    const int ahead = far ? shared_len - k0 : -k0;
-    f32x4 s[NB][2] = {};
+  for (int tile = from + wave; tile < to; tile += NT * WV) {
+    f32x4 s[NB][2 * NT] = {};
+    int k0[NT], end[NT], ahead[NT];
+    bool far[NT], near = false, cut = false;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int u = 0; u < NT; ++u) {
+      const int at = tile + u * WV;
+      far[u] = at < far_tiles;
+      k0[u] = (far[u] ? at : at - far_tiles) * KT;
+      end[u] = at < to ? (far[u] ? shared_len : own_len) : 0;
+      // distance of a query at own row pos from key 0 of the tile: shared rows stand before the own ones
+      ahead[u] = far[u] ? shared_len - k0[u] : -k0[u];
+      near |= biased && lowest + ahead[u] - (KT - 1) < reach;
+      cut |= k0[u] + KT > end[u] || (!far[u] && k0[u] + KT > lowest + 1);
 #pragma unroll
-      for (int f = 0; f < KS; ++f) {
-        const frag_t<T> kf = fl.key(t, f);
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int n = 0; n < NB; ++n) s[n][t] = mma16(kf, qf[n][f], s[n][t]);
-      }
-    fl.put_v(vt, min(end - k0, KT), lane);
-    if (tile + WAVES < to) fetch(tile + WAVES);
-    const bool near = biased && lowest + ahead - (KT - 1) < reach;
-    const bool cut = k0 + KT > end || (!far && k0 + KT > lowest + 1);
-    frag_t<T> pf[NB];
+        for (int i = 0; i < KS; ++i) {
+          const frag_t<T> kf = fl[u].key(t, i);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) s[n][2 * u + t] = mma16(kf, qf[n][i], s[n][2 * u + t]);
+        }
+      fl[u].put_v(vt + u * TB, min(end[u] - k0[u], KT), lane);
+    }
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+      if (tile + (NT + u) * WV < to) fetch(fl[u], tile + (NT + u) * WV);
+    frag_t<T> pf[NB][NT];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      float x[8];
+      float x[8 * NT];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __builtin_fmaf(s[n][j >> 2][j & 3], scale2, near ? 0.f : farthest[n]);
+      for (int j = 0; j < 8 * NT; ++j) x[j] = __builtin_fmaf(s[n][j >> 2][j & 3], scale2, near ? 0.f : farthest[n]);
       if (near) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += bias[mine[n] + min(max(pos[n] + ahead - 8 * g - j, 0), reach)];
+        for (int j = 0; j < 8 * NT; ++j) x[j] += bias[mine[n] + min(max(pos[n] + ahead[j >> 3] - 8 * g - (j & 7), 0), reach)];
       }
       if (cut) {
-        const int seen = far ? end : min(end, pos[n] + 1);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k0 + 8 * g + j >= seen) x[j] = -INFINITY;
+        for (int j = 0; j < 8 * NT; ++j)
+          if (k0[j >> 3] + 8 * g + (j & 7) >= (far[j >> 3] ? end[j >> 3] : min(end[j >> 3], pos[n] + 1))) x[j] = -INFINITY;
       }
       float top = x[0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+      for (int j = 1; j < 8 * NT; ++j) top = fmaxf(top, x[j]);
       if (__any(top > m[n] + SLACK)) {       // exponentials up to 2^SLACK are as good as up to 1: the maximum seldom moves
         const float now = fmaxf(m[n], max_groups(top));
         const float keep = now == -INFINITY ? 1.f : exp2_(m[n] - now);
@@ -274,29 +309,62 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
           for (int r = 0; r < 4; ++r) o[n][d][r] *= keep;
       }
       const float base = m[n] == -INFINITY ? 0.f : m[n];
-      f32x8 e;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[j] = exp2_(x[j] - base);
-        l[n] += e[j];
+      for (int u = 0; u < NT; ++u) {
+        f32x8 e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] = exp2_(x[8 * u + j] - base);
+          l[n] += e[j];
+        }
+        pf[n][u] = to_frag<T>(e);
       }
-      pf[n] = to_frag<T>(e);
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const frag_t<T> vf = TL::col_frag(vt, 8 * g, 16 * d, lane);
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int n = 0; n < NB; ++n) o[n][d] = mma16(vf, pf[n], o[n][d]);
-    }
+      for (int u = 0; u < NT; ++u) {
+        const frag_t<T> vf = TL::col_frag(vt + u * TB, 8 * g, 16 * d, lane);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) o[n][d] = mma16(vf, pf[n][u], o[n][d]);
+      }
     __builtin_amdgcn_wave_barrier();
   }
 
+  // Results: of this piece, [shared rows' | own rows'] [row][piece][D + 4] = unnormalised output, maximum, sum; or the outputs.
+  auto put = [&](int r, int e, f32x4 x, float top, float sum) {
+    if (p.direct) {
+      const int sub = shared ? r / per : 0, in = r - sub * per, gi = p.t == 1 ? in : in / p.t;
+      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] *= inv;
+      const long at = (((long)(shared ? unit * p.each + sub : unit) * p.t + in - gi * p.t) * p.h + kvh * p.group + gi) * D + 4 * e;
+      *reinterpret_cast<vec4_t<T> *>(reinterpret_cast<T *>(p.out) + at) = to_vec4<T>(x);
+    } else {
+      const long base_row = shared ? 0 : (long)p.shared_splits * p.b * p.hkv * per;
+      float *to_ = p.part + (base_row + (((long)unit * p.hkv + kvh) * rows + r) * splits + piece) * (D + 4);
+      *reinterpret_cast<f32x4 *>(to_ + 4 * e) = x;
+      if (e == 0) { to_[D] = top; to_[D + 1] = sum; }
+    }
+  };
+  if constexpr (WV == 1) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float sum = sum_groups(l[n]);
+      const bool live = pos[n] >= 0;                                        // what is no query has seen the shared rows for nothing
+      if (r0 + 16 * n + col < rows)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) put(r0 + 16 * n + col, 4 * d + g, live ? o[n][d] : f32x4{}, live ? m[n] : -INFINITY, live ? sum : 0.f);
+    }
+    return;
+  }
   // join the four waves, one block of 16 rows at a time: a wave leaves its output, scaled to the common maximum, in LDS
   float *mine_o = reinterpret_cast<float *>(lds);                           // [WAVES][16][D]; the V tiles are done with
+  float *stat = bias + biases;                                              // [2][WAVES][16]
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const bool live = pos[n] >= 0;                                          // what is no query has seen the shared rows for nothing
+    const bool live = pos[n] >= 0;
     const float sum = live ? sum_groups(l[n]) : 0.f;
     if (!live) m[n] = -INFINITY;
     __syncthreads();
@@ -334,31 +402,23 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
 #pragma unroll
         for (int q = 0; q < 4; ++q) x[q] += y[q];
       }
-      const float rt_max = stat[c], rt_sum = stat[WAVES * 16 + c];
-      if (p.direct) {
-        const int in = r % per, seq = shared ? unit * p.each + r / per : unit;
-        const float inv = rt_sum > 0.f || rt_sum != rt_sum ? 1.f / rt_sum : 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) x[q] *= inv;
-        const long at = (((long)seq * p.t + in % p.t) * p.h + kvh * p.group + in / p.t) * D + 4 * e;
-        *reinterpret_cast<vec4_t<T> *>(reinterpret_cast<T *>(p.out) + at) = to_vec4<T>(x);
-      } else {
-        // pieces of a row lie side by side: [shared rows' | own rows'] [row][piece][D + 2]
-        const long base_row = shared ? 0 : (long)p.shared_splits * p.b * p.hkv * per;
-        float *to_ = p.part + (base_row + (((long)unit * p.hkv + kvh) * rows + r) * splits + piece) * (D + 4);
-        *reinterpret_cast<f32x4 *>(to_ + 4 * e) = x;
-        if (e == 0) { to_[D] = rt_max; to_[D + 1] = rt_sum; }
-      }
+      put(r, e, x, stat[c], stat[WAVES * 16 + c]);
     }
   }
 }
 
-// Two waves a SIMD: a wave's loads hide behind another one's arithmetic (f32 keeps its registers: 512 a lane).
-template <typename T, int D, bool Q, int NB>
-__global__ __launch_bounds__(WAVES * 64, sizeof(T) == 2 ? 2 : 1) void decode_kernel(const DecodeParams p) {
+// Waves a SIMD: a wave's loads hide behind another one's arithmetic (f32 keeps its registers: 512 a lane).
+template <typename T> constexpr int resident(int d) { return sizeof(T) == 4 ? 1 : d == 64 ? 3 : 2; }
+
+template <typename T, int D, bool Q, int NB, int WV>
+__global__ __launch_bounds__(WAVES * 64, resident<T>(D)) void decode_kernel(const DecodeParams p) {
   extern __shared__ __align__(16) char lds[];
-  if ((int)blockIdx.x < p.shared_items) walk<T, D, Q, NB>(p, blockIdx.x, true, lds);
-  else walk<T, D, Q, 1>(p, blockIdx.x - p.shared_items, false, lds);
+  if ((int)blockIdx.x < p.shared_items) {
+    walk<T, D, Q, NB, WAVES>(p, blockIdx.x, true, lds);
+  } else {
+    const int item = (blockIdx.x - p.shared_items) * (WAVES / WV) + (WV == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    if (item < p.own_items) walk<T, D, Q, 1, WV>(p, item, false, lds);
+  }
 }
 
 // Joins the pieces of a row, shared ones first.  A wave owns a row: lane i weighs piece i (64 at a time), then groups of D / 4
@@ -436,7 +496,10 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) 
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
-struct Plan { int nb, own_splits, shared_splits, own_tiles, shared_tiles, shared_items, own_items, bias_heads, joined, direct; size_t lds; };
+struct Plan {
+  int nb, wv, own_splits, shared_splits, own_tiles, shared_tiles, shared_items, own_items, own_heads, shared_heads, joined, direct;
+  size_t lds;
+};
 
 int check(const char *where, const sig3d_decode_attention_args *a) {
   LANG_NEED(where, a != nullptr, "no arguments");
@@ -451,8 +514,9 @@ int check(const char *where, const sig3d_decode_attention_args *a) {
   return check_buckets(where, a->buckets, a->table, a->table_rows);
 }
 
-// Blocks of 16 query rows a workgroup takes over shared keys: what two waves a SIMD leave registers for.
-constexpr int blocks_of_rows(int dtype, int d) { return dtype != 0 && d == 64 ? 4 : 2; }
+// Blocks of 16 query rows a workgroup takes over shared keys: what leaves registers for two waves a SIMD and more (four blocks:
+// 64 questions over 5000 shared rows, 64 wide, took 39 us instead of 36).
+constexpr int BLOCKS = 2;
 
 Plan plan(const sig3d_decode_attention_args *a) {
   Plan s = {};
@@ -468,24 +532,31 @@ Plan plan(const sig3d_decode_attention_args *a) {
   s.own_splits = (int)std::min<long>(std::max<long>(1, 4096 / base), sig3d_ceil_div(own_rows, LEAST * KT));
   if (each > 0 && !s.joined) {
     const long rows = (long)each * per;
-    s.nb = rows > 16 ? blocks_of_rows(a->dtype, a->d) : 1;
+    s.nb = rows > 16 ? BLOCKS : 1;
     s.shared_tiles = sig3d_ceil_div(rows, 16 * s.nb);
     const long far = (long)a->groups * a->hkv * s.shared_tiles;
-    s.shared_splits = (int)std::min<long>(std::max<long>(1, 2048 / far), sig3d_ceil_div(a->shared_capacity, LEAST * KT));
+    s.shared_splits = (int)std::min<long>(std::max<long>(1, 768 / far), sig3d_ceil_div(a->shared_capacity, LEAST * KT));
     s.shared_items = (int)(far * s.shared_splits);
   }
   s.own_items = (int)(base * s.own_splits);
   s.direct = s.own_splits == 1 && !s.shared_splits;
   const int e = a->dtype == 0 ? 4 : 2, row = (a->d * e / 16 + 7) / 8 * 8 * 16;
-  s.bias_heads = a->buckets.n ? std::min(group, (16 * s.nb + a->t - 2) / a->t + 1) : 0;
-  s.lds = std::max<size_t>(WAVES * KT * row, WAVES * 16 * a->d * 4) + (size_t)s.bias_heads * (reach + 1) * 4 + 2 * WAVES * 16 * 4;
+  if (a->buckets.n) {
+    s.own_heads = std::min(group, (16 + a->t - 2) / a->t + 1);
+    s.shared_heads = s.shared_splits ? std::min(group, (16 * s.nb + a->t - 2) / a->t + 1) : 0;
+  }
+  // One wave an item where a sequence is short: four would start and join for a tile or two each.
+  const size_t one = (size_t)WAVES * s.own_heads * (reach + 1) * 4;
+  s.wv = one <= 32 * 1024 && (own_rows <= 2 * KT || (base >= 1024 && own_rows <= 16 * KT)) ? 1 : WAVES;
+  s.lds = WAVES * KT * row * (a->d == 64 && e == 2 ? 2 : 1) + std::max(s.wv == 1 ? one : s.own_heads * (reach + 1) * 4ul, s.shared_heads * (reach + 1) * 4ul) +
+          2 * WAVES * 16 * 4;
   return s;
 }
 
-template <typename T, int D, bool Q, int NB> int launch(const DecodeParams &p, const Plan &s, hipStream_t stream) {
+template <typename T, int D, bool Q, int NB, int WV> int launch(const DecodeParams &p, const Plan &s, hipStream_t stream) {
   static sig3d_once_per_device once;
-  if (int e = allow_lds(decode_kernel<T, D, Q, NB>, once)) return e;
-  decode_kernel<T, D, Q, NB><<<s.shared_items + s.own_items, WAVES * 64, s.lds, stream>>>(p);
+  if (int e = allow_lds(decode_kernel<T, D, Q, NB, WV>, once)) return e;
+  decode_kernel<T, D, Q, NB, WV><<<s.shared_items + sig3d_ceil_div(s.own_items, WAVES / WV), WAVES * 64, s.lds, stream>>>(p);
   SIG3D_LAUNCH_CHECK("decode_kernel");
   if (!p.direct) {
     decode_join_kernel<T, D><<<sig3d_ceil_div((long)p.b * p.h * p.t, 4), 256, 0, stream>>>(p);
@@ -527,14 +598,23 @@ extern "C" int sig3d_decode_attention(const sig3d_decode_attention_args *a, void
   p.b = a->b; p.t = a->t; p.h = a->h; p.hkv = a->hkv; p.group = a->h / a->hkv;
   p.each = a->groups ? a->b / a->groups : 0;
   p.own_splits = s.own_splits; p.shared_splits = s.shared_splits; p.own_tiles = s.own_tiles; p.shared_tiles = s.shared_tiles;
-  p.shared_items = s.shared_items; p.bias_heads = s.bias_heads; p.joined = s.joined; p.direct = s.direct;
+  p.own_items = s.own_items; p.shared_items = s.shared_items; p.own_bias_heads = s.own_heads; p.shared_bias_heads = s.shared_heads;
+  p.joined = s.joined; p.direct = s.direct;
   p.scale = a->scale;
   p.bk = device_buckets(a->buckets);
   return by_type(a->dtype, a->d, [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
-    constexpr int NB = blocks_of_rows(sizeof(T) == 4 ? 0 : 1, D);
-    if (s.nb == NB) return quantized ? launch<T, D, true, NB>(p, s, (hipStream_t)stream) : launch<T, D, false, NB>(p, s, (hipStream_t)stream);
-    return quantized ? launch<T, D, true, 1>(p, s, (hipStream_t)stream) : launch<T, D, false, 1>(p, s, (hipStream_t)stream);
+    const auto go = [&](auto q, auto nb, auto wv) {
+      return launch<T, D, decltype(q)::value, decltype(nb)::value, decltype(wv)::value>(p, s, (hipStream_t)stream);
+    };
+    const auto by_rows = [&](auto q) {
+      const std::integral_constant<int, 1> one;
+      const std::integral_constant<int, BLOCKS> some;
+      const std::integral_constant<int, WAVES> all;
+      if (s.nb == 1) return s.wv == 1 ? go(q, one, one) : go(q, one, all);
+      return s.wv == 1 ? go(q, some, one) : go(q, some, all);
+    };
+    return quantized ? by_rows(std::true_type()) : by_rows(std::false_type());
   });
 }

@@ -170,16 +170,16 @@ template <typename T, int D> struct Tile {
 
 // ---- relative position buckets -----------------------------------------------------------------------------------------
 // One direction has n buckets; border[i] is the smallest distance of bucket i (host-made from whole numbers), and from
-// distance `reach` = border of the last bucket on nothing changes any more.
+// distance `reach` = border of the last bucket on nothing changes any more.  of[a]: the bucket of distance a <= reach, so that
+// a kernel finds it with one load (counting borders costs 3 instructions each, for every wave of every workgroup).
 struct Buckets {
   int n, reach, both;      // both: keys ahead of the query have buckets n .. 2 n - 1 of their own; else they share bucket 0
-  int border[SIG3D_REL_MAX_BUCKETS];
+  short border[SIG3D_REL_MAX_BUCKETS];
+  unsigned char of[SIG3D_REL_MAX_REACH + 4];
 };
-__device__ __forceinline__ int bucket_of(const Buckets &bk, int relative) {
+__device__ __forceinline__ int bucket_of(const Buckets &bk, int relative) {      // |relative| <= reach
   const int a = relative < 0 ? -relative : (bk.both ? relative : 0);
-  int i = -1;
-  for (int j = 0; j < bk.n; ++j) i += a >= bk.border[j] ? 1 : 0;
-  return i + (bk.both && relative > 0 ? bk.n : 0);
+  return bk.of[a] + (bk.both && relative > 0 ? bk.n : 0);
 }
 // by_distance[r + reach] = log2(e) * table[bucket(r)][head] for r in [-reach, reach]
 template <typename T>
@@ -216,7 +216,12 @@ inline Buckets device_buckets(const sig3d_rel_buckets &k) {
   d.n = k.n;
   d.both = k.both;
   if (k.n > 0) d.reach = k.border[k.n - 1] > 0 ? k.border[k.n - 1] : 1;
-  for (int i = 0; i < k.n; ++i) d.border[i] = k.border[i];
+  for (int i = 0; i < k.n; ++i) d.border[i] = (short)k.border[i];
+  if (k.n > 0)
+    for (int a = 0, i = 0; a <= d.reach; ++a) {
+      while (i + 1 < k.n && k.border[i + 1] <= a) ++i;
+      d.of[a] = (unsigned char)i;
+    }
   return d;
 }
 
