@@ -101,7 +101,7 @@ template <typename T, int D, bool Q> struct Flight {
     }
   }
   static __device__ __forceinline__ void put_piece(char *tile, int r, int o, frag_t<T> x) {
-    typedef Tile<T, D> TL;
+    typedef Tile<T, D, true> TL;
     if constexpr (sizeof(T) == 2) {
       *reinterpret_cast<frag_t<T> *>(tile + TL::at(r, o)) = x;
     } else {
@@ -147,7 +147,7 @@ template <typename T, int D> constexpr int TILES = D == 64 && sizeof(T) == 2 ? 2
 // through LDS) or by one wave alone.
 template <typename T, int D, bool Q, int NB, int WV>
 __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool shared, char *lds) {
-  typedef Tile<T, D> TL;
+  typedef Tile<T, D, true> TL;
   typedef Flight<T, D, Q> FL;
   constexpr int KS = FL::KS, TB = KT * TL::ROW, DT = D / 16;
   // tiles a step: a lone wave has nobody to hide its latencies behind but its own second tile
@@ -540,7 +540,7 @@ Plan plan(const sig3d_decode_attention_args *a) {
   }
   s.own_items = (int)(base * s.own_splits);
   s.direct = s.own_splits == 1 && !s.shared_splits;
-  const int e = a->dtype == 0 ? 4 : 2, row = (a->d * e / 16 + 7) / 8 * 8 * 16;
+  const int e = a->dtype == 0 ? 4 : 2, row = a->d * e + 32;
   if (a->buckets.n) {
     s.own_heads = std::min(group, (16 + a->t - 2) / a->t + 1);
     s.shared_heads = s.shared_splits ? std::min(group, (16 * s.nb + a->t - 2) / a->t + 1) : 0;
@@ -548,6 +548,7 @@ Plan plan(const sig3d_decode_attention_args *a) {
   // One wave an item where a sequence is short: four would start and join for a tile or two each.
   const size_t one = (size_t)WAVES * s.own_heads * (reach + 1) * 4;
   s.wv = one <= 32 * 1024 && (own_rows <= 2 * KT || (base >= 1024 && own_rows <= 16 * KT)) ? 1 : WAVES;
+  // (the V tiles also hold the four waves' outputs while they join: 16 rows of d floats each, less)
   s.lds = WAVES * KT * row * (a->d == 64 && e == 2 ? 2 : 1) + std::max(s.wv == 1 ? one : s.own_heads * (reach + 1) * 4ul, s.shared_heads * (reach + 1) * 4ul) +
           2 * WAVES * 16 * 4;
   return s;

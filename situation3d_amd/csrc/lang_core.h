@@ -130,12 +130,17 @@ template <> __device__ __forceinline__ f16x8 from_e4m3<_Float16>(uint2 w, float 
 // [rows][D] of T in 16-byte chunks; chunk c of a row sits at c ^ swz(row).  swz separates, inside a 128-byte bank window,
 // the eight rows that eight consecutive lanes of a fragment read touch (kappa order: 0-3, 8-11), and the four rows of a
 // 16-lane group of a transposing read (32 bytes each).  Rows of 12 chunks (96 x 2 bytes) are padded to 16.
-template <typename T, int D> struct Tile {
+// PAD: a tile that is only read transposed has its rows 32 bytes further apart instead: the four rows of a group are as far
+// apart, and every address is a lane's base plus a constant.
+template <typename T, int D, bool PAD = false> struct Tile {
   static constexpr int CH = D * (int)sizeof(T) / 16;        // chunks of data in a row
-  static constexpr int CHP = (CH + 7) / 8 * 8;              // chunks stored
+  static constexpr int CHP = PAD ? CH + 2 : (CH + 7) / 8 * 8;       // chunks stored
   static constexpr int ROW = CHP * 16;                      // bytes
-  static __device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 3) & 1); }
-  static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW + ((chunk ^ swz(row)) << 4); }
+  static __device__ __forceinline__ int swz(int row) { return PAD ? 0 : ((row & 3) << 1) | ((row >> 3) & 1); }
+  // (the upper bits of a chunk stay out of the exclusive or: they are constants of an unrolled loop, and of the instruction)
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return row * ROW + (((chunk & 7) ^ swz(row)) << 4) + ((chunk & ~7) << 4);
+  }
 
   // elements 8 o .. 8 o + 7 of a row
   static __device__ __forceinline__ frag_t<T> row_frag(const char *t, int row, int o) {
