@@ -186,12 +186,17 @@ __device__ __forceinline__ int bucket_of(const Buckets &bk, int relative) {     
   const int a = relative < 0 ? -relative : (bk.both ? relative : 0);
   return bk.of[a] + (bk.both && relative > 0 ? bk.n : 0);
 }
-// by_distance[r + reach] = log2(e) * table[bucket(r)][head] for r in [-reach, reach]
+// by_distance[r + reach + EDGE] = log2(e) * table[bucket(r)][head], for r in [-reach - EDGE, reach + EDGE]: a tile that any
+// distance below `reach` touches stays inside, so that nobody clamps an index
+constexpr int EDGE = 96;
+__host__ __device__ constexpr int bias_floats(int reach) { return 2 * (reach + EDGE) + 1; }
 template <typename T>
 __device__ __forceinline__ void fill_bias(float *by_distance, const Buckets &bk, const T *table, int heads, int head, int tid,
                                           int threads) {
-  for (int i = tid; i <= 2 * bk.reach; i += threads)
-    by_distance[i] = (float)table[(long)bucket_of(bk, i - bk.reach) * heads + head] * LOG2E;
+  for (int i = tid; i < bias_floats(bk.reach); i += threads) {
+    const int r = min(max(i - bk.reach - EDGE, -bk.reach), bk.reach);
+    by_distance[i] = (float)table[(long)bucket_of(bk, r) * heads + head] * LOG2E;
+  }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------

@@ -121,6 +121,7 @@ __device__ __forceinline__ void store_row(T *row, const f32x16 (&acc)[D / 32], f
 }
 
 template <typename T> constexpr bool narrow() { return std::is_same<T, _Float16>::value; }
+constexpr float SLACK = 8.f;                  // of the forward pass's reference value (see there)
 constexpr int P_UP = 8, DS_UP = 3;            // f16: exponents that P and dS are raised by (see the top)
 
 template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
@@ -129,11 +130,15 @@ template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32
 // column, i.e. register r stands at relative position first + sign * (16 (r >> 3) + (r & 7)).
 template <int SIGN>
 __device__ __forceinline__ void add_bias(f32x16 &s, const float *by_distance, int reach, int first) {
+  const float *b = by_distance + first + reach + EDGE;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int rel = first + SIGN * (16 * (r >> 3) + (r & 7));
-    s[r] += by_distance[min(max(rel, -reach), reach) + reach];
-  }
+  for (int r = 0; r < 16; ++r) s[r] += b[SIGN * (16 * (r >> 3) + (r & 7))];
+}
+
+// Where a block of keys [k0, k0 + n) stands for queries at positions [p0, p0 + 32): wholly behind or ahead of `reach`, or near.
+enum Where { NEAR, BEHIND, AHEAD };
+__device__ __forceinline__ Where where(int k0, int n, int p0, int reach) {
+  return k0 + n - 1 - p0 <= -reach ? BEHIND : k0 - (p0 + 31) >= reach ? AHEAD : NEAR;
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
@@ -178,6 +183,8 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
   const float scale2 = p.scale * LOG2E;
   const int reach = p.bk.reach, qpos = qi + p.offset, q0pos = (qt * NW + wave) * 32 + p.offset;
 
+  const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
+
   f32x16 o[D / 32] = {};
   float m = -INFINITY, l = 0.f;
   const int first = wlo < whi ? wlo / KT * KT : 0;
@@ -207,17 +214,24 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
           s[u] = mma32(TL::row_frag(kt, u * 32 + kappa(col), 2 * f + half), qf[f], s[u]);
       }
       float add = 0.f;
-      bool near = false;
+      bool plain = scale2 >= 0.f && t >= sp.all_lo && t + KT <= sp.all_hi;      // no mask, no bias but one: nothing per element
       if (biased) {
-        const int nearest_lo = t - (q0pos + 31), nearest_hi = t + KT - 1 - q0pos;
-        near = nearest_hi > -reach && nearest_lo < reach;
-        if (!near) add = nearest_hi <= -reach ? bias[0] : bias[2 * reach];
-      }
+        const Where w = where(t, KT, q0pos, reach);
+        if (w == NEAR) plain = false;
+        else add = w == BEHIND ? bias_behind : bias_ahead;
+        if (!plain) {
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) {
+          for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], scale2, add);
-        if (near) add_bias<1>(s[u], bias, reach, t + u * 32 + 8 * half - qpos);
+            for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(s[u][r], scale2, add);
+            if (w == NEAR) add_bias<1>(s[u], bias, reach, t + u * 32 + 8 * half - qpos);
+          }
+        }
+      } else if (!plain) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[u][r] *= scale2;
       }
       if (t < sp.all_lo || t + KT > sp.all_hi) {
 #pragma unroll
@@ -231,9 +245,11 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-      top = max_halves(top);
-      if (__any(top > m)) {                                  // the running maximum rarely moves after the first tiles
-        const float now = fmaxf(m, top);
+      if (plain) top = __builtin_fmaf(top, scale2, add);
+      // The reference value m follows the running maximum only when a score passes it by 2^SLACK: exponentials up to that are as
+      // good as up to 1 (f32 sums; a rounding is relative), and rescaling the output costs as much as a third of a tile.
+      if (__any(top > m + SLACK)) {
+        const float now = fmaxf(m, max_halves(top));
         const float keep = now == -INFINITY ? 1.f : exp2_(m - now);
         m = now;
         l *= keep;
@@ -243,11 +259,12 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
           for (int r = 0; r < 16; ++r) o[blk][r] *= keep;
       }
       const float base = m == -INFINITY ? 0.f : m;
+      const float factor = plain ? scale2 : 1.f, offset = plain ? add - base : -base;
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[u][r] = exp2_(s[u][r] - base);
+          s[u][r] = exp2_(__builtin_fmaf(s[u][r], factor, offset));
           l += s[u][r];
         }
 #pragma unroll
@@ -283,17 +300,20 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
 // ---- backward: dQ, delta, the table's gradient ------------------------------------------------------------------------------
 // Same tiling as the forward pass (a query is a lane): P = exp2(s - lse), dP^T = V dO^T, dS = P (dP - delta) with
 // delta = dO.O from the unrounded O, dQ^T = K^T dS^T.
-// Table: dS summed by distance.  Beyond `reach` everything falls into the end buckets: two registers.  Along the diagonal
-// each wave adds its dS into its own LDS row of 2 reach + 1 distances; one instruction adds the 32 lanes of one half, whose
-// distances differ, so no two lanes meet at an address and the order of the sums is that of the program.
+// Table: dS summed by distance.  Beyond `reach` everything falls into the end buckets: two registers.  A 32 x 32 block along
+// the diagonal goes through wave-private LDS, one row of 36 floats a distance, element (query i, key j) at [j - i + 31][i]: the
+// addresses are a lane's base plus constants, and lane l then adds row l and puts the sum to its distance -- 64 distances, 64
+// lanes, no two meet and the order of the sums is fixed.  (Adding every element to its distance by an LDS atomic cost 200
+// address and mask instructions and twice the LDS time: 88 us instead of DQ_US for 4 x 32 heads of 432 tokens.)
+constexpr int DIAG_ROW = 36, DIAG = 64 * DIAG_ROW;        // floats; 36: 16-byte rows whose columns spread over the banks
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
   extern __shared__ __align__(16) char lds[];
   float *bias = reinterpret_cast<float *>(lds + 4 * TB);
-  const int reach = p.bk.reach, span = 2 * reach + 1;
-  float *sums = bias + span;                              // [NW][span]
+  const int reach = p.bk.reach, span = bias_floats(reach);
+  float *sums = bias + (span + 3) / 4 * 4;                // [NW][span]
   __shared__ int ends[2][NW];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
@@ -344,7 +364,7 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
   const bool biased = p.bk.n > 0;
   if (biased) {
     fill_bias(bias, p.bk, reinterpret_cast<const T *>(p.table), p.h, head, tid, NT);
-    for (int i = tid; i < NW * span; i += NT) sums[i] = 0.f;
+    for (int i = tid; i < NW * ((span + 3) / 4 * 4 + DIAG); i += NT) sums[i] = 0.f;
   }
   __syncthreads();
   int wlo = INT_MAX, whi = 0;
@@ -358,7 +378,10 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
   const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
   const float scale2 = p.scale * LOG2E;
   const int qpos = qi + p.offset, q0pos = (qt * NW + wave) * 32 + p.offset;
-  float *mine = sums + wave * span;
+  float *mine = sums + wave * ((span + 3) / 4 * 4), *diag = sums + NW * ((span + 3) / 4 * 4) + wave * DIAG;
+  // element of register 0: key 8 half, query col; lane l reads distance l - 31
+  float *const diag_put = diag + (8 * half - col + 31) * DIAG_ROW + col, *const diag_get = diag + lane * DIAG_ROW;
+  const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
 
   f32x16 dq[D / 32] = {};
   float behind = 0.f, ahead = 0.f;
@@ -389,21 +412,18 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
           s = mma32(TL::row_frag(kt, u * 32 + kappa(col), 2 * f + half), qf[f], s);
           dp = mma32(TL::row_frag(vt, u * 32 + kappa(col), 2 * f + half), gf[f], dp);
         }
-        float add = 0.f;
-        bool near = false, left = false;
-        if (biased) {
-          const int nearest_lo = t + u * 32 - (q0pos + 31), nearest_hi = t + u * 32 + 31 - q0pos;
-          left = nearest_hi <= -reach;
-          near = !left && nearest_lo < reach;
-          if (!near) add = left ? bias[0] : bias[2 * reach];
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, add);
+        const Where w = biased ? where(t + u * 32, 32, q0pos, reach) : BEHIND;
         const int rel0 = t + u * 32 + 8 * half - qpos;
-        if (near) add_bias<1>(s, bias, reach, rel0);
+        if (w == NEAR) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] = exp2_(s[r] - lse) * (dp[r] - delta);
+          for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, -lse);
+          add_bias<1>(s, bias, reach, rel0);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = exp2_(s[r]) * (dp[r] - delta);
+        } else {
+          const float add = (w == BEHIND ? bias_behind : bias_ahead) - lse;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], scale2, add)) * (dp[r] - delta);
         }
         if (cut) {
 #pragma unroll
@@ -411,22 +431,25 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
             if ((unsigned)(t + u * 32 + reg_row(r, half) - lo) >= (unsigned)(hi - lo)) s[r] = 0.f;
         }
         if (biased) {
-          if (near) {
+          if (w == NEAR) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int rel = rel0 + 16 * (r >> 3) + (r & 7);
-              if (rel <= -reach) behind += s[r] * undo;
-              else if (rel >= reach) ahead += s[r] * undo;
-              else {
-                if (half == 0) __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float *)(mine + rel + reach), s[r] * undo, 0, 0, false);
-                if (half == 1) __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float *)(mine + rel + reach), s[r] * undo, 0, 0, false);
-              }
-            }
+            for (int r = 0; r < 16; ++r) diag_put[(16 * (r >> 3) + (r & 7)) * DIAG_ROW] = narrow<T>() ? s[r] * undo : s[r];
+            __builtin_amdgcn_wave_barrier();
+            f32x4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const f32x4 *>(diag_get + 4 * i);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
+            mine[t + u * 32 - q0pos - 31 + lane + reach + EDGE] += sum;
+            __builtin_amdgcn_wave_barrier();
           } else {
             float x = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) x += s[r];
-            (left ? behind : ahead) += x * undo;
+            if (narrow<T>()) x *= undo;
+            if (w == BEHIND) behind += x;
+            else ahead += x;
           }
         }
 #pragma unroll
@@ -452,27 +475,26 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
   const float far_behind = wave_allreduce_sum_f32(behind), far_ahead = wave_allreduce_sum_f32(ahead);
   if (lane == 0) {
     mine[0] += far_behind;
-    mine[2 * reach] += far_ahead;
+    mine[2 * (reach + EDGE)] += far_ahead;
   }
   __syncthreads();
   // distances -> buckets (keys ahead share bucket 0 unless they have their own), one row of partial sums a workgroup
   float *part = p.hist + ((long)bh * p.qtiles + qt) * p.table_rows;
+  const int pitch = (span + 3) / 4 * 4, most = reach + EDGE;
   for (int bucket = tid; bucket < p.table_rows; bucket += NT) {
     float x = 0.f;
-    const bool second = p.bk.both && bucket >= p.bk.n && bucket < 2 * p.bk.n, first_dir = bucket < p.bk.n;
-    if (first_dir || second) {
-      const int i = second ? bucket - p.bk.n : bucket;
-      const int from = p.bk.border[i], to = i + 1 < p.bk.n ? p.bk.border[i + 1] : reach + 1;      // distances [from, to)
-      for (int a = from; a < to; ++a) {
-        if (second ? a == 0 : false) continue;
-        const int at = second ? reach + a : reach - a;
+    const auto add = [&](int from, int to) {               // relative positions [from, to]
+      for (int a = from; a <= to; ++a)
 #pragma unroll
-        for (int w = 0; w < NW; ++w) x += sums[w * span + at];
-      }
-      if (!second && !p.bk.both && i == 0)
-        for (int a = 1; a <= reach; ++a)
-#pragma unroll
-          for (int w = 0; w < NW; ++w) x += sums[w * span + reach + a];
+        for (int w = 0; w < NW; ++w) x += sums[w * pitch + a + most];
+    };
+    const bool second = p.bk.both && bucket >= p.bk.n && bucket < 2 * p.bk.n;
+    const int i = second ? bucket - p.bk.n : bucket;
+    if (bucket < p.bk.n || second) {
+      const int from = p.bk.border[i], to = i + 1 < p.bk.n ? p.bk.border[i + 1] - 1 : most;
+      if (second) add(max(from, 1), to);
+      else add(-to, -from);
+      if (i == 0 && !p.bk.both) add(1, most);
     }
     part[bucket] = x;
   }
@@ -618,16 +640,16 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dkv_kernel(const Params p) {
             dp = mma32(TL::row_frag(gt, u * 32 + kappa(col), 2 * f + half), vf[f], dp);
           }
           const int p0 = q0 + u * 32 + p.offset;
-          float add = 0.f;
-          bool near = false;
-          if (biased) {
-            const int nearest_lo = kw - (p0 + 31), nearest_hi = kw + 31 - p0;
-            near = nearest_hi > -reach && nearest_lo < reach;
-            if (!near) add = nearest_hi <= -reach ? bias[0] : bias[2 * reach];
-          }
+          const Where w = biased ? where(kw, 32, p0, reach) : BEHIND;
+          if (w == NEAR) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, add);
-          if (near) add_bias<-1>(s, bias, reach, key - (p0 + 8 * half));
+            for (int r = 0; r < 16; ++r) s[r] *= scale2;
+            add_bias<-1>(s, bias, reach, key - (p0 + 8 * half));
+          } else {
+            const float add = biased ? bias[w == BEHIND ? 0 : 2 * (reach + EDGE)] : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale2, add);
+          }
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const int at = u * 32 + 16 * g + 8 * half;
@@ -717,7 +739,7 @@ long work_hist(const sig3d_rel_attention_args *a) {
 
 template <typename T, int D> int launch_fwd(const Params &p, hipStream_t stream) {
   static sig3d_once_per_device once;
-  const size_t lds = 4 * key_tile<T>() * Tile<T, D>::ROW + (2 * p.bk.reach + 1) * sizeof(float);
+  const size_t lds = 4 * key_tile<T>() * Tile<T, D>::ROW + bias_floats(p.bk.reach) * sizeof(float);
   if (int e = allow_lds(rel_fwd_kernel<T, D, NW>, once)) return e;
   rel_fwd_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, lds, stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_fwd_kernel");
@@ -726,11 +748,11 @@ template <typename T, int D> int launch_fwd(const Params &p, hipStream_t stream)
 
 template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream) {
   static sig3d_once_per_device once_q, once_kv;
-  const int span = 2 * p.bk.reach + 1;
+  const int span = (bias_floats(p.bk.reach) + 3) / 4 * 4;
   const size_t tiles = 4 * key_tile<T>() * Tile<T, D>::ROW;
   if (int e = allow_lds(rel_bwd_dq_kernel<T, D, NW>, once_q)) return e;
   if (int e = allow_lds(rel_bwd_dkv_kernel<T, D, NW>, once_kv)) return e;
-  rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, tiles + (NW + 1) * span * sizeof(float), stream>>>(p);
+  rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, tiles + ((NW + 1) * span + NW * DIAG) * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dq_kernel");
   rel_bwd_dkv_kernel<T, D, NW><<<p.b * p.hkv * p.ktiles, NW * 64, tiles + span * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dkv_kernel");
