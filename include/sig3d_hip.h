@@ -855,7 +855,7 @@ int sig3d_bn_relu_bwd_compact(int b, int c, long e, int p, const float *dA, cons
  * The operators of the language head behind the point branch (blip2_t5.py:102-183; its attention is modeling_t5.py's): the
  * reference runs them as torch operations over a materialised (b, h, nq, nk) score and bias tensor.
  * dtype: 0 float32, 1 bfloat16, 2 float16.  Every tensor is dense in its innermost dimension; the strides given here are in
- * elements; addresses and strides (in bytes) are multiples of 16.  d: 64, 96 or 128; h a multiple of hkv, head i reads key
+ * elements; addresses and strides (in bytes) are multiples of 16, a token's stride is below 16 MB.  d: 64, 96 or 128; h a multiple of hkv, head i reads key
  * head i / (h / hkv).  No call records a memset node; results do not depend on the order in which workgroups run.  The _work_floats functions return -1 for arguments
  * that the calls refuse. */
 #define SIG3D_REL_MAX_BUCKETS 128   /* of one direction */

@@ -72,24 +72,29 @@ __device__ __forceinline__ int xcd_contiguous(int id, int total) {
   return id < each * 8 ? (id & 7) * each + (id >> 3) : id;
 }
 
-// Rows [row0, row0 + ROWS) of a token-major operand through registers into an LDS tile; rows outside [lo, hi) become zero.
+// Rows [row0, row0 + ROWS) of a token-major operand through registers into an LDS tile; rows outside [lo, hi) become zero.  Their
+// loads repeat the nearest row inside (no branch: a load under a condition is waited for at once, and the next tile's loads
+// are to be in flight while this one is used); `store` clears them, which only tiles at an end pay for.
 template <typename T, int D, int ROWS, int NT> struct Stage {
   typedef Tile<T, D> TL;
   static constexpr int N = (ROWS * TL::CH + NT - 1) / NT;
   u32x4 r[N];
   __device__ __forceinline__ void load(const T *base, long stride, int row0, int lo, int hi, int tid) {
+    const char *tile = reinterpret_cast<const char *>(base + (long)row0 * stride);      // one scalar address, 32-bit offsets
+    const int first = max(lo - row0, 0), last = min(hi - 1 - row0, ROWS - 1);
+    const unsigned pitch = (unsigned)stride * (unsigned)sizeof(T);                       // below 2^24: the host looks
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = tid + i * NT, row = c / TL::CH, ch = c - row * TL::CH;
-      r[i] = u32x4{0, 0, 0, 0};
-      if ((ROWS * TL::CH % NT == 0 || row < ROWS) && row0 + row >= lo && row0 + row < hi)
-        r[i] = *reinterpret_cast<const u32x4 *>(base + (long)(row0 + row) * stride + ch * (16 / (int)sizeof(T)));
+      r[i] = *reinterpret_cast<const u32x4 *>(tile + (__umul24((unsigned)min(max(row, first), last), pitch) + (unsigned)ch * 16u));
     }
   }
-  __device__ __forceinline__ void store(char *tile, int tid) const {
+  __device__ __forceinline__ void store(char *tile, int row0, int lo, int hi, int tid) {
+    const bool whole = row0 >= lo && row0 + ROWS <= hi;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = tid + i * NT, row = c / TL::CH, ch = c - row * TL::CH;
+      if (!whole && (row0 + row < lo || row0 + row >= hi)) r[i] = u32x4{0, 0, 0, 0};
       if (ROWS * TL::CH % NT == 0 || row < ROWS) *reinterpret_cast<u32x4 *>(tile + TL::at(row, ch)) = r[i];
     }
   }
@@ -146,7 +151,7 @@ __device__ __forceinline__ Where where(int k0, int n, int p0, int reach) {
 // the next tile's loads are in flight while the current one is used, one barrier a tile.
 // S^T = K Q^T, then O^T = V^T P^T: a query is one lane (and lane ^ 32), its softmax is in-lane work.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void rel_fwd_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
   extern __shared__ __align__(16) char lds[];
@@ -192,8 +197,8 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
   if (wlo < whi) {
     ks.load(kb, p.k_n, first, wlo, whi, tid);
     vs.load(vb, p.v_n, first, wlo, whi, tid);
-    ks.store(lds, tid);
-    vs.store(lds + TB, tid);
+    ks.store(lds, first, wlo, whi, tid);
+    vs.store(lds + TB, first, wlo, whi, tid);
   }
   __syncthreads();
   int buf = 0;
@@ -280,8 +285,8 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
       }
     }
     if (more) {
-      ks.store(lds + (buf ^ 1) * 2 * TB, tid);
-      vs.store(lds + (buf ^ 1) * 2 * TB + TB, tid);
+      ks.store(lds + (buf ^ 1) * 2 * TB, t + KT, wlo, whi, tid);
+      vs.store(lds + (buf ^ 1) * 2 * TB + TB, t + KT, wlo, whi, tid);
     }
     __syncthreads();
   }
@@ -307,7 +312,7 @@ __global__ __launch_bounds__(NW * 64) void rel_fwd_kernel(const Params p) {
 // address and mask instructions and twice the LDS time: 88 us instead of DQ_US for 4 x 32 heads of 432 tokens.)
 constexpr int DIAG_ROW = 36, DIAG = 64 * DIAG_ROW;        // floats; 36: 16-byte rows whose columns spread over the banks
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void rel_bwd_dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
   extern __shared__ __align__(16) char lds[];
@@ -390,8 +395,8 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
   if (wlo < whi) {
     ks.load(kb, p.k_n, first, wlo, whi, tid);
     vs.load(vb, p.v_n, first, wlo, whi, tid);
-    ks.store(lds, tid);
-    vs.store(lds + TB, tid);
+    ks.store(lds, first, wlo, whi, tid);
+    vs.store(lds + TB, first, wlo, whi, tid);
   }
   __syncthreads();
   int buf = 0;
@@ -465,8 +470,8 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dq_kernel(const Params p) {
       }
     }
     if (more) {
-      ks.store(lds + (buf ^ 1) * 2 * TB, tid);
-      vs.store(lds + (buf ^ 1) * 2 * TB + TB, tid);
+      ks.store(lds + (buf ^ 1) * 2 * TB, t + KT, wlo, whi, tid);
+      vs.store(lds + (buf ^ 1) * 2 * TB + TB, t + KT, wlo, whi, tid);
     }
     __syncthreads();
   }
@@ -521,7 +526,7 @@ __global__ __launch_bounds__(256) void rel_bwd_table_kernel(const float *hist, i
 // lse, delta, intervals).  S = Q K^T, dP = dO V^T with queries along the registers: P and dS are at once the B operands of
 // dV^T += dO^T P and dK^T += Q^T dS.  The heads that share the keys are a loop: their sums stay in the accumulators.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void rel_bwd_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void rel_bwd_dkv_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int QT = key_tile<T>(), NT = NW * 64, SUB = QT / 32, TB = QT * TL::ROW;
   extern __shared__ __align__(16) char lds[];
@@ -613,9 +618,9 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dkv_kernel(const Params p) {
           }
         }
       };
-      auto put = [&](int buf) {
-        qs.store(lds + buf * 2 * TB, tid);
-        gs.store(lds + buf * 2 * TB + TB, tid);
+      auto put = [&](int buf, int tile) {
+        qs.store(lds + buf * 2 * TB, tile * QT, 0, p.nq, tid);
+        gs.store(lds + buf * 2 * TB + TB, tile * QT, 0, p.nq, tid);
         if (tid < QT) {
           stats[buf][0][tid] = st; stats[buf][1][tid] = dl;
           rows[buf][0][tid] = rlo; rows[buf][1][tid] = rhi - rlo;
@@ -623,7 +628,7 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dkv_kernel(const Params p) {
       };
       if (n > 0) {
         fetch(todo[0] & ~(1 << 30));
-        put(0);
+        put(0, todo[0] & ~(1 << 30));
       }
       __syncthreads();
       for (int i = 0; i < n; ++i) {
@@ -676,7 +681,7 @@ __global__ __launch_bounds__(NW * 64) void rel_bwd_dkv_kernel(const Params p) {
             }
           }
         }
-        if (i + 1 < n) put(buf ^ 1);
+        if (i + 1 < n) put(buf ^ 1, todo[i + 1] & ~(1 << 30));
         __syncthreads();
       }
     }
@@ -701,6 +706,8 @@ int check(const char *where, const sig3d_rel_attention_args *a) {
   const int e = a->dtype == 0 ? 4 : 2;
   const long strides[9] = {a->q_b, a->q_n, a->q_h, a->k_b, a->k_n, a->k_h, a->v_b, a->v_n, a->v_h};
   for (long s : strides) LANG_NEED(where, s >= 0 && s * e % 16 == 0, "strides must be non-negative multiples of 16 bytes");
+  const long rows[3] = {a->q_n, a->k_n, a->v_n};
+  for (long s : rows) LANG_NEED(where, s * e < (1l << 24), "token strides must be below 16 MB");
   LANG_NEED(where, a->q && a->k && a->v && a->out && aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->out),
        "q, k, v, out must be 16-byte aligned addresses");
   LANG_NEED(where, (a->out32 == nullptr) == (a->lse == nullptr) && aligned16(a->out32), "out32 and lse come together");
@@ -786,7 +793,8 @@ extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *
   SIG3D_REQUIRE(aligned16(a->grad) && aligned16(a->dq) && aligned16(a->dk) && aligned16(a->dv) && aligned16(a->work),
                 "addresses must be 16-byte aligned");
   SIG3D_REQUIRE(a->grad_b >= 0 && a->grad_n >= 0 && a->grad_h >= 0 && a->grad_b * e % 16 == 0 && a->grad_n * e % 16 == 0 &&
-                    a->grad_h * e % 16 == 0, "strides must be non-negative multiples of 16 bytes");
+                    a->grad_h * e % 16 == 0 && a->grad_n * e < (1l << 24),
+                "strides must be non-negative multiples of 16 bytes, that of a token below 16 MB");
   SIG3D_REQUIRE(a->buckets.n == 0 || a->dtable, "a bias needs dtable");
   Params p = params(a);
   p.delta = a->work;

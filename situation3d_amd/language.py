@@ -68,7 +68,7 @@ def _dense_rows(t):
     for _ in range(2):
         e = t.element_size()
         strides = [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
-        if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in strides):
+        if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in strides) and strides[1] * e < 1 << 24:
             return t, strides
         t = t.clone(memory_format=torch.contiguous_format)
     raise RuntimeError("could not lay out a tensor of shape %s" % (tuple(t.shape),))
