@@ -190,14 +190,26 @@ __device__ __forceinline__ int bucket_of(const Buckets &bk, int relative) {     
 // distance below `reach` touches stays inside, so that nobody clamps an index
 constexpr int EDGE = 96;
 __host__ __device__ constexpr int bias_floats(int reach) { return 2 * (reach + EDGE) + 1; }
-template <typename T>
-__device__ __forceinline__ void fill_bias(float *by_distance, const Buckets &bk, const T *table, int heads, int head, int tid,
-                                          int threads) {
-  for (int i = tid; i < bias_floats(bk.reach); i += threads) {
+// `start` sends a thread's first load out (two in a row: bucket, entry), `finish` puts the values where they belong: between
+// the two there is time for everything else that a workgroup loads before it begins.
+template <typename T> struct BiasFill {
+  float first = 0.f;
+  static __device__ __forceinline__ float value(const Buckets &bk, const T *table, int heads, int head, int i) {
     const int r = min(max(i - bk.reach - EDGE, -bk.reach), bk.reach);
-    by_distance[i] = (float)table[(long)bucket_of(bk, r) * heads + head] * LOG2E;
+    return (float)table[(long)bucket_of(bk, r) * heads + head] * LOG2E;
   }
-}
+  __device__ __forceinline__ void start(const Buckets &bk, const void *table, int heads, int head, int tid) {
+    if (bk.n > 0) first = value(bk, reinterpret_cast<const T *>(table), heads, head, min(tid, bias_floats(bk.reach) - 1));
+  }
+  __device__ __forceinline__ void finish(float *by_distance, const Buckets &bk, const void *table, int heads, int head, int tid,
+                                         int threads) const {
+    if (bk.n <= 0) return;
+    const int n = bias_floats(bk.reach);
+    if (tid < n) by_distance[tid] = first;
+    for (int i = tid + threads; i < n; i += threads)
+      by_distance[i] = value(bk, reinterpret_cast<const T *>(table), heads, head, i);
+  }
+};
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
 #define LANG_NEED(where, cond, msg)               \

@@ -100,15 +100,12 @@ template <typename T, int D, int ROWS, int NT> struct Stage {
   }
 };
 
-// fragment f of a stationary row: elements 16 f + 8 half .. + 7; zero when the row does not exist
+// fragment f of a stationary row: elements 16 f + 8 half .. + 7  (rows that do not exist repeat the last one: a lane that has
+// one takes part in nothing but its own column)
 template <typename T, int D>
-__device__ __forceinline__ void load_row(frag_t<T> (&f)[D / 16], const T *row, int half, bool valid) {
+__device__ __forceinline__ void load_row(frag_t<T> (&f)[D / 16], const T *row, int half) {
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
-    frag_t<T> x{};
-    if (valid) x = *reinterpret_cast<const frag_t<T> *>(row + 16 * s + 8 * half);
-    f[s] = x;
-  }
+  for (int s = 0; s < D / 16; ++s) f[s] = *reinterpret_cast<const frag_t<T> *>(row + 16 * s + 8 * half);
 }
 
 // A (D x 32) accumulator whose columns are rows of a dense tensor: registers 4 g .. 4 g + 3 are four consecutive elements.
@@ -162,6 +159,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;      // causal: the long rows first
   const int b = bh / p.h, head = bh - b * p.h;
+  BiasFill<T> fill;
+  fill.start(p.bk, p.table, p.h, head, tid);
   const int qi = (qt * NW + wave) * 32 + col;
   const bool valid = qi < p.nq;
   int lo = 0, hi = 0;
@@ -171,10 +170,6 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
     ends[0][wave] = sp.any_lo;
     ends[1][wave] = sp.any_hi;
   }
-  frag_t<T> qf[D / 16];
-  load_row<T, D>(qf, reinterpret_cast<const T *>(p.q) + b * p.q_b + (long)qi * p.q_n + head * p.q_h, half, valid);
-  const bool biased = p.bk.n > 0;
-  if (biased) fill_bias(bias, p.bk, reinterpret_cast<const T *>(p.table), p.h, head, tid, NT);
   __syncthreads();
   int wlo = INT_MAX, whi = 0;
 #pragma unroll
@@ -187,20 +182,24 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
   const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
   const float scale2 = p.scale * LOG2E;
   const int reach = p.bk.reach, qpos = qi + p.offset, q0pos = (qt * NW + wave) * 32 + p.offset;
-
-  const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
-
-  f32x16 o[D / 32] = {};
-  float m = -INFINITY, l = 0.f;
   const int first = wlo < whi ? wlo / KT * KT : 0;
   Stage<T, D, KT, NT> ks, vs;
   if (wlo < whi) {
     ks.load(kb, p.k_n, first, wlo, whi, tid);
     vs.load(vb, p.v_n, first, wlo, whi, tid);
+  }
+  frag_t<T> qf[D / 16];
+  load_row<T, D>(qf, reinterpret_cast<const T *>(p.q) + b * p.q_b + (long)min(qi, p.nq - 1) * p.q_n + head * p.q_h, half);
+  fill.finish(bias, p.bk, p.table, p.h, head, tid, NT);
+  if (wlo < whi) {
     ks.store(lds, first, wlo, whi, tid);
     vs.store(lds + TB, first, wlo, whi, tid);
   }
+  f32x16 o[D / 32] = {};
+  float m = -INFINITY, l = 0.f;
   __syncthreads();
+  const bool biased = p.bk.n > 0;
+  const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
   int buf = 0;
   for (int t = first; t < whi; t += KT, buf ^= 1) {
     const bool more = t + KT < whi;
@@ -325,6 +324,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void r
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;
   const int b = bh / p.h, head = bh - b * p.h;
+  BiasFill<T> fill;
+  fill.start(p.bk, p.table, p.h, head, tid);
   const int qi = (qt * NW + wave) * 32 + col;
   const bool valid = qi < p.nq;
   int lo = 0, hi = 0;
@@ -335,21 +336,36 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void r
     ends[1][wave] = sp.any_hi;
     if (head == 0) p.blocks[((long)b * p.qtiles + qt) * NW + wave] = make_int4(sp.any_lo, sp.any_hi, sp.all_lo, sp.all_hi);
   }
+  __syncthreads();
+  int wlo = INT_MAX, whi = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    wlo = min(wlo, ends[0][w]);
+    whi = max(whi, ends[1][w]);
+  }
+  const int kvh = head / p.group;
+  const T *kb = reinterpret_cast<const T *>(p.k) + b * p.k_b + kvh * p.k_h;
+  const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
+  const int first = wlo < whi ? wlo / KT * KT : 0;
+  Stage<T, D, KT, NT> ks, vs;
+  if (wlo < whi) {
+    ks.load(kb, p.k_n, first, wlo, whi, tid);
+    vs.load(vb, p.v_n, first, wlo, whi, tid);
+  }
   frag_t<T> qf[D / 16], gf[D / 16];
-  load_row<T, D>(qf, reinterpret_cast<const T *>(p.q) + b * p.q_b + (long)qi * p.q_n + head * p.q_h, half, valid);
-  load_row<T, D>(gf, reinterpret_cast<const T *>(p.grad) + b * p.grad_b + (long)qi * p.grad_n + head * p.grad_h, half, valid);
-  const long row = (((long)b * p.nq + qi) * p.h + head) * D, stat = ((long)b * p.h + head) * p.nq + qi;
-  float delta = 0.f, lse = INFINITY;
-  if (valid) {
-    lse = p.lse[stat];
+  const int qrow = min(qi, p.nq - 1);
+  load_row<T, D>(qf, reinterpret_cast<const T *>(p.q) + b * p.q_b + (long)qrow * p.q_n + head * p.q_h, half);
+  load_row<T, D>(gf, reinterpret_cast<const T *>(p.grad) + b * p.grad_b + (long)qrow * p.grad_n + head * p.grad_h, half);
+  const long row = (((long)b * p.nq + qrow) * p.h + head) * D, stat = ((long)b * p.h + head) * p.nq + qrow;
+  float delta = 0.f, lse = p.lse[stat];
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const f32x8 x = *reinterpret_cast<const f32x8 *>(p.out32 + row + 16 * s + 8 * half);
+  for (int s = 0; s < D / 16; ++s) {
+    const f32x8 x = *reinterpret_cast<const f32x8 *>(p.out32 + row + 16 * s + 8 * half);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[s][j], x[j], delta);
-    }
+    for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[s][j], x[j], delta);
   }
   delta = sum_halves(delta);
+  if (!valid) lse = INFINITY;
   if (valid && half == 0) p.delta[stat] = delta;
   float undo = 1.f;                                       // dS is held times 1 / undo
   if constexpr (narrow<T>()) {
@@ -368,37 +384,22 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void r
   }
   const bool biased = p.bk.n > 0;
   if (biased) {
-    fill_bias(bias, p.bk, reinterpret_cast<const T *>(p.table), p.h, head, tid, NT);
-    for (int i = tid; i < NW * ((span + 3) / 4 * 4 + DIAG); i += NT) sums[i] = 0.f;
+    fill.finish(bias, p.bk, p.table, p.h, head, tid, NT);
+    for (int i = tid; i < NW * ((span + 3) / 4 + DIAG / 4); i += NT) reinterpret_cast<f32x4 *>(sums)[i] = f32x4{};
   }
-  __syncthreads();
-  int wlo = INT_MAX, whi = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    wlo = min(wlo, ends[0][w]);
-    whi = max(whi, ends[1][w]);
+  if (wlo < whi) {
+    ks.store(lds, first, wlo, whi, tid);
+    vs.store(lds + TB, first, wlo, whi, tid);
   }
-  const int kvh = head / p.group;
-  const T *kb = reinterpret_cast<const T *>(p.k) + b * p.k_b + kvh * p.k_h;
-  const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
   const float scale2 = p.scale * LOG2E;
   const int qpos = qi + p.offset, q0pos = (qt * NW + wave) * 32 + p.offset;
   float *mine = sums + wave * ((span + 3) / 4 * 4), *diag = sums + NW * ((span + 3) / 4 * 4) + wave * DIAG;
   // element of register 0: key 8 half, query col; lane l reads distance l - 31
   float *const diag_put = diag + (8 * half - col + 31) * DIAG_ROW + col, *const diag_get = diag + lane * DIAG_ROW;
-  const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
-
   f32x16 dq[D / 32] = {};
   float behind = 0.f, ahead = 0.f;
-  const int first = wlo < whi ? wlo / KT * KT : 0;
-  Stage<T, D, KT, NT> ks, vs;
-  if (wlo < whi) {
-    ks.load(kb, p.k_n, first, wlo, whi, tid);
-    vs.load(vb, p.v_n, first, wlo, whi, tid);
-    ks.store(lds, first, wlo, whi, tid);
-    vs.store(lds + TB, first, wlo, whi, tid);
-  }
   __syncthreads();
+  const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
   int buf = 0;
   for (int t = first; t < whi; t += KT, buf ^= 1) {
     const bool more = t + KT < whi;
@@ -483,15 +484,21 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void r
     mine[2 * (reach + EDGE)] += far_ahead;
   }
   __syncthreads();
-  // distances -> buckets (keys ahead share bucket 0 unless they have their own), one row of partial sums a workgroup
+  // distances -> buckets (keys ahead share bucket 0 unless they have their own), one row of partial sums a workgroup: the
+  // waves' rows are added first, then a wave takes every fourth bucket, its lanes the distances
   float *part = p.hist + ((long)bh * p.qtiles + qt) * p.table_rows;
   const int pitch = (span + 3) / 4 * 4, most = reach + EDGE;
-  for (int bucket = tid; bucket < p.table_rows; bucket += NT) {
+  for (int i = tid; i < span; i += NT) {
+    float x = sums[i];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) x += sums[w * pitch + i];
+    sums[i] = x;
+  }
+  __syncthreads();
+  for (int bucket = wave; bucket < p.table_rows; bucket += NW) {
     float x = 0.f;
     const auto add = [&](int from, int to) {               // relative positions [from, to]
-      for (int a = from; a <= to; ++a)
-#pragma unroll
-        for (int w = 0; w < NW; ++w) x += sums[w * pitch + a + most];
+      for (int a = from + lane; a <= to; a += 64) x += sums[a + most];
     };
     const bool second = p.bk.both && bucket >= p.bk.n && bucket < 2 * p.bk.n;
     const int i = second ? bucket - p.bk.n : bucket;
@@ -501,7 +508,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void r
       else add(-to, -from);
       if (i == 0 && !p.bk.both) add(1, most);
     }
-    part[bucket] = x;
+    x = wave_allreduce_sum_f32(x);
+    if (lane == 0) part[bucket] = x;
   }
 }
 
@@ -543,8 +551,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void re
   const int k0 = kt0 * NW * 32, kw = k0 + wave * 32, key = kw + col;
   const bool valid = key < p.nk;
   frag_t<T> kf[D / 16], vf[D / 16];
-  load_row<T, D>(kf, reinterpret_cast<const T *>(p.k) + b * p.k_b + (long)key * p.k_n + kvh * p.k_h, half, valid);
-  load_row<T, D>(vf, reinterpret_cast<const T *>(p.v) + b * p.v_b + (long)key * p.v_n + kvh * p.v_h, half, valid);
+  const int krow = min(key, p.nk - 1);
+  load_row<T, D>(kf, reinterpret_cast<const T *>(p.k) + b * p.k_b + (long)krow * p.k_n + kvh * p.k_h, half);
+  load_row<T, D>(vf, reinterpret_cast<const T *>(p.v) + b * p.v_b + (long)krow * p.v_n + kvh * p.v_h, half);
   const bool biased = p.bk.n > 0;
   const float scale2 = p.scale * LOG2E;
   const int nblocks = (p.nq + 31) / 32, ntiles = (p.nq + QT - 1) / QT;
@@ -568,10 +577,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void re
 
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
   for (int head = kvh * p.group; head < (kvh + 1) * p.group; ++head) {
-    if (biased) {
-      __syncthreads();
-      fill_bias(bias, p.bk, reinterpret_cast<const T *>(p.table), p.h, head, tid, NT);
-    }
+    BiasFill<T> fill;
+    fill.start(p.bk, p.table, p.h, head, tid);
+    __syncthreads();
+    fill.finish(bias, p.bk, p.table, p.h, head, tid, NT);
     const T *qb = reinterpret_cast<const T *>(p.q) + b * p.q_b + head * p.q_h;
     const T *gb = reinterpret_cast<const T *>(p.grad) + b * p.grad_b + head * p.grad_h;
     const long stat = ((long)b * p.h + head) * p.nq;
