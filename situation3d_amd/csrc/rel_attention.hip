@@ -20,6 +20,8 @@
 
 #include <limits.h>
 
+#include <algorithm>
+
 namespace {
 using namespace lang;
 
@@ -28,10 +30,11 @@ struct Params {
   const int *key_lengths, *prefix_lengths, *key_ranges;
   void *out, *dq, *dk, *dv, *dtable;
   float *out32, *lse, *delta, *hist;
+  float *part;                                // backward: dK, dV of every split, (2, splits, b, nk, hkv, d), or NULL: one split
   int4 *blocks;                               // backward: interval summary of every 32 queries
   int *tops;                                  // backward, f16: exponent of the largest |dO| of a head's 32 queries
   long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, grad_b, grad_n, grad_h;
-  int b, nq, nk, h, hkv, group, causal, offset, table_rows, qtiles, ktiles;
+  int b, nq, nk, h, hkv, group, causal, offset, table_rows, qtiles, ktiles, head_splits, query_splits;
   float scale;
   Buckets bk;
 };
@@ -532,7 +535,9 @@ __global__ __launch_bounds__(256) void rel_bwd_table_kernel(const float *hist, i
 // ---- backward: dK, dV --------------------------------------------------------------------------------------------------------
 // A wave owns 32 keys (columns; K and V rows in registers), a workgroup NW waves that share the streamed query tiles (Q, dO,
 // lse, delta, intervals).  S = Q K^T, dP = dO V^T with queries along the registers: P and dS are at once the B operands of
-// dV^T += dO^T P and dK^T += Q^T dS.  The heads that share the keys are a loop: their sums stay in the accumulators.
+// dV^T += dO^T P and dK^T += Q^T dS.  The heads that share the keys are a loop: their sums stay in the accumulators -- unless
+// there are too few workgroups for the chip (see splits_of): then heads and runs of queries become workgroups of their own,
+// which leave f32 sums that a small kernel adds in order.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void rel_bwd_dkv_kernel(const Params p) {
   typedef Tile<T, D> TL;
@@ -546,8 +551,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void re
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bh = id / p.ktiles, kt0 = id % p.ktiles;
+  const int splits = p.head_splits * p.query_splits, split = id % splits, tile_id = id / splits;
+  const int bh = tile_id / p.ktiles, kt0 = tile_id % p.ktiles;
   const int b = bh / p.hkv, kvh = bh - b * p.hkv;
+  const int heads = p.group / p.head_splits, head0 = kvh * p.group + split / p.query_splits * heads;
   const int k0 = kt0 * NW * 32, kw = k0 + wave * 32, key = kw + col;
   const bool valid = key < p.nk;
   frag_t<T> kf[D / 16], vf[D / 16];
@@ -576,7 +583,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void re
   const float ds_factor = __builtin_ldexpf(1.f, up - (narrow<T>() ? P_UP : 0));
 
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
-  for (int head = kvh * p.group; head < (kvh + 1) * p.group; ++head) {
+  const int run = (ntiles + p.query_splits - 1) / p.query_splits;
+  const int tile0 = split % p.query_splits * run, tile1 = min(tile0 + run, ntiles);
+  for (int head = head0; head < head0 + heads; ++head) {
     BiasFill<T> fill;
     fill.start(p.bk, p.table, p.h, head, tid);
     __syncthreads();
@@ -584,15 +593,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void re
     const T *qb = reinterpret_cast<const T *>(p.q) + b * p.q_b + head * p.q_h;
     const T *gb = reinterpret_cast<const T *>(p.grad) + b * p.grad_b + head * p.grad_h;
     const long stat = ((long)b * p.h + head) * p.nq;
-    for (int chunk = 0; chunk < ntiles; chunk += 256) {
+    for (int chunk = tile0; chunk < tile1; chunk += 256) {
       // query tiles that see any of these keys, in order; bit 30: some query does not see all of them
       __syncthreads();
       if (wave == 0) {
         int n = 0;
-        for (int c = chunk; c < min(chunk + 256, ntiles); c += 64) {
+        for (int c = chunk; c < min(chunk + 256, tile1); c += 64) {
           const int tile = c + lane;
           bool any = false, cut = false;
-          if (tile < ntiles) {
+          if (tile < tile1) {
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
               const int blk = tile * SUB + u;
@@ -697,8 +706,30 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void re
   }
   if (!valid) return;
   const long row = (((long)b * p.nk + key) * p.hkv + kvh) * D;
+  if (p.part) {
+    const long all = (long)p.b * p.nk * p.hkv * D;
+    store_row<float, D>(p.part + split * all + row, dk, p.scale * __builtin_ldexpf(1.f, -up), half);
+    store_row<float, D>(p.part + (splits + split) * all + row, dv, narrow<T>() ? 1.f / (1 << P_UP) : 1.f, half);
+    return;
+  }
   store_row<T, D>(reinterpret_cast<T *>(p.dk) + row, dk, p.scale * __builtin_ldexpf(1.f, -up), half);
   store_row<T, D>(reinterpret_cast<T *>(p.dv) + row, dv, narrow<T>() ? 1.f / (1 << P_UP) : 1.f, half);
+}
+
+// dK, dV = the sums of their splits, in order
+template <typename T>
+__global__ __launch_bounds__(256) void rel_bwd_fold_kernel(const float *part, int splits, long quads, T *dk, T *dv) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads) return;
+  const f32x4 *from = reinterpret_cast<const f32x4 *>(part) + (long)blockIdx.y * splits * quads + i;
+  f32x4 x = from[0];
+#pragma unroll 4
+  for (int s = 1; s < splits; ++s) {
+    const f32x4 y = from[s * quads];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += y[e];
+  }
+  reinterpret_cast<vec4_t<T> *>(blockIdx.y ? dv : dk)[i] = to_vec4<T>(x);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------------------
@@ -721,7 +752,7 @@ int check(const char *where, const sig3d_rel_attention_args *a) {
        "q, k, v, out must be 16-byte aligned addresses");
   LANG_NEED(where, (a->out32 == nullptr) == (a->lse == nullptr) && aligned16(a->out32), "out32 and lse come together");
   if (int e = check_buckets(where, a->buckets, a->table, a->table_rows)) return e;
-  LANG_NEED(where, (long)a->b * a->h * ((a->nq + 31) / 32) < INT_MAX && (long)a->b * a->h * ((a->nk + 31) / 32) < INT_MAX, "grid too large");
+  LANG_NEED(where, (long)a->b * a->h * ((a->nq + 31) / 32) < INT_MAX && (long)a->b * a->h * ((a->nk + 31) / 32) < INT_MAX / 16, "grid too large");
   return 0;
 }
 
@@ -747,10 +778,31 @@ Params params(const sig3d_rel_attention_args *a) {
 long work_delta(const sig3d_rel_attention_args *a) { return ((long)a->b * a->h * a->nq + 3) / 4 * 4; }
 long work_blocks(const sig3d_rel_attention_args *a) { return (long)a->b * sig3d_ceil_div(a->nq, NW * 32) * NW * 4; }
 long work_tops(const sig3d_rel_attention_args *a) {
-  return a->dtype == 2 ? (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * NW : 0;
+  return a->dtype == 2 ? ((long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * NW + 3) / 4 * 4 : 0;
 }
 long work_hist(const sig3d_rel_attention_args *a) {
   return a->buckets.n > 0 ? (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * a->table_rows : 0;
+}
+
+// Splits of the dK / dV kernel.  Causal and packed rows make workgroups very unequal -- the first keys of a document are seen by
+// all of it -- so there should be several for every CU (4 for each of 256); a run of queries is worth a workgroup from 8 tiles
+// on.  A split costs a write and a read of 8 bytes an element of dK and dV.  (2 x 4096 packed tokens, 16 heads on 4, 128 wide:
+// 524 us as 256 workgroups.)
+struct Splits { int heads, queries; };
+Splits splits_of(const sig3d_rel_attention_args *a) {
+  const long base = (long)a->b * a->hkv * sig3d_ceil_div(a->nk, NW * 32);
+  const int want = (int)std::min<long>(16, (1024 + base - 1) / base), group = a->h / a->hkv;
+  Splits s = {1, 1};
+  for (int n = 2; n <= want; ++n)
+    if (group % n == 0) s.heads = n;
+  const int tiles = sig3d_ceil_div(a->nq, a->dtype == 0 ? 32 : 64);
+  s.queries = std::max(1, std::min(want / s.heads, tiles / 8));
+  return s;
+}
+long work_part(const sig3d_rel_attention_args *a) {
+  const Splits s = splits_of(a);
+  const long n = (long)s.heads * s.queries;
+  return n > 1 ? 2 * n * a->b * a->nk * a->hkv * a->d : 0;
 }
 
 template <typename T, int D> int launch_fwd(const Params &p, hipStream_t stream) {
@@ -770,8 +822,14 @@ template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream)
   if (int e = allow_lds(rel_bwd_dkv_kernel<T, D, NW>, once_kv)) return e;
   rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, tiles + ((NW + 1) * span + NW * DIAG) * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dq_kernel");
-  rel_bwd_dkv_kernel<T, D, NW><<<p.b * p.hkv * p.ktiles, NW * 64, tiles + span * sizeof(float), stream>>>(p);
+  rel_bwd_dkv_kernel<T, D, NW><<<p.b * p.hkv * p.ktiles * p.head_splits * p.query_splits, NW * 64, tiles + span * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dkv_kernel");
+  if (p.part) {
+    const long quads = (long)p.b * p.nk * p.hkv * D / 4;
+    rel_bwd_fold_kernel<T><<<dim3(sig3d_ceil_div(quads, 256), 2), 256, 0, stream>>>(
+        p.part, p.head_splits * p.query_splits, quads, reinterpret_cast<T *>(p.dk), reinterpret_cast<T *>(p.dv));
+    SIG3D_LAUNCH_CHECK("rel_bwd_fold_kernel");
+  }
   if (p.bk.n > 0) {
     rel_bwd_table_kernel<T><<<dim3(p.h, sig3d_ceil_div(p.table_rows, 4)), 256, 0, stream>>>(
         p.hist, p.b, p.h, p.qtiles, p.table_rows, reinterpret_cast<T *>(p.dtable));
@@ -792,7 +850,7 @@ extern "C" int sig3d_rel_attention_fwd(const sig3d_rel_attention_args *a, void *
 
 extern "C" long sig3d_rel_attention_bwd_work_floats(const sig3d_rel_attention_args *a) {
   if (check("sig3d_rel_attention_bwd_work_floats", a)) return -1;
-  return work_delta(a) + work_blocks(a) + work_tops(a) + work_hist(a);
+  return work_delta(a) + work_blocks(a) + work_tops(a) + (work_hist(a) + 3) / 4 * 4 + work_part(a);
 }
 
 extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *stream) {
@@ -810,6 +868,10 @@ extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *
   p.blocks = reinterpret_cast<int4 *>(a->work + work_delta(a));
   p.tops = reinterpret_cast<int *>(a->work + work_delta(a) + work_blocks(a));
   p.hist = a->work + work_delta(a) + work_blocks(a) + work_tops(a);
+  const Splits s = splits_of(a);
+  p.head_splits = s.heads;
+  p.query_splits = s.queries;
+  if (s.heads * s.queries > 1) p.part = p.hist + (work_hist(a) + 3) / 4 * 4;
   return by_type(a->dtype, a->d, [&](auto t, auto d) {
     return launch_bwd<decltype(t), decltype(d)::value>(p, (hipStream_t)stream);
   });
