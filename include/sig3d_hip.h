@@ -907,8 +907,14 @@ typedef struct {
 } sig3d_cache_append_args;
 int sig3d_cache_append(const sig3d_cache_append_args *args, void *stream);
 /* k_out / v_out (b, n, hkv, d) dense, of dtype: the values that the first n rows hold, zeros from lengths[b] on */
-int sig3d_cache_read(int dtype, int b, int n, int capacity, int hkv, int d, const void *k_cache, const void *v_cache,
-                     const float *k_scale, const float *v_scale, const int *lengths, void *k_out, void *v_out, void *stream);
+typedef struct {
+  const void *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int *lengths;
+  void *k_out, *v_out;
+  int dtype, b, n, capacity, hkv, d;
+} sig3d_cache_read_args;
+int sig3d_cache_read(const sig3d_cache_read_args *args, void *stream);
 
 /* Attention of new tokens over the cache they have been appended to.  Sequence i sees the rows of shared sequence
  * i / (b / groups), [0, shared_lengths[.]), then its own: with n = counts[i] (default t) new tokens, query j < n is the token

@@ -276,6 +276,12 @@ class CacheAppendArgs(ctypes.Structure):
                 + [(n, _I) for n in ("dtype", "b", "t", "capacity", "hkv", "d")])
 
 
+class CacheReadArgs(ctypes.Structure):
+    """sig3d_cache_read_args of include/sig3d_hip.h."""
+    _fields_ = ([(n, _P) for n in ("k_cache", "v_cache", "k_scale", "v_scale", "lengths", "k_out", "v_out")]
+                + [(n, _I) for n in ("dtype", "b", "n", "capacity", "hkv", "d")])
+
+
 class DecodeAttentionArgs(ctypes.Structure):
     """sig3d_decode_attention_args of include/sig3d_hip.h."""
     _fields_ = ([(n, _P) for n in ("q", "table", "k_cache", "v_cache", "shared_k", "shared_v", "k_scale", "v_scale",
@@ -288,7 +294,7 @@ class DecodeAttentionArgs(ctypes.Structure):
 SIGNATURES["sig3d_rel_attention_fwd"] = [ctypes.POINTER(RelAttentionArgs), _P]
 SIGNATURES["sig3d_rel_attention_bwd"] = [ctypes.POINTER(RelAttentionArgs), _P]
 SIGNATURES["sig3d_cache_append"] = [ctypes.POINTER(CacheAppendArgs), _P]
-SIGNATURES["sig3d_cache_read"] = [_I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["sig3d_cache_read"] = [ctypes.POINTER(CacheReadArgs), _P]
 SIGNATURES["sig3d_decode_attention"] = [ctypes.POINTER(DecodeAttentionArgs), _P]
 
 

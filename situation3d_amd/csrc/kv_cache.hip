@@ -189,20 +189,20 @@ extern "C" int sig3d_cache_append(const sig3d_cache_append_args *a, void *stream
   return 0;
 }
 
-extern "C" int sig3d_cache_read(int dtype, int b, int n, int capacity, int hkv, int d, const void *k_cache, const void *v_cache,
-                                const float *k_scale, const float *v_scale, const int *lengths, void *k_out, void *v_out,
-                                void *stream) {
-  if (int e = check_cache("sig3d_cache_read", dtype, b, capacity, hkv, d)) return e;
-  SIG3D_REQUIRE(n >= 1 && n <= capacity && (long)n * d < (1l << 33), "row count out of range");
-  SIG3D_REQUIRE(k_cache && v_cache && lengths && k_out && v_out, "missing array");
-  SIG3D_REQUIRE((k_scale == nullptr) == (v_scale == nullptr), "k_scale and v_scale come together");
-  SIG3D_REQUIRE(aligned16(k_cache) && aligned16(v_cache) && aligned16(k_out) && aligned16(v_out), "addresses must be 16-byte aligned");
-  const ReadParams p = {k_cache, v_cache, k_scale, v_scale, lengths, k_out, v_out, n, capacity, hkv};
-  const dim3 grid(sig3d_ceil_div((long)n * (d / 8), 256), hkv, b);
-  return by_type(dtype, d, [&](auto t, auto dd) {
+extern "C" int sig3d_cache_read(const sig3d_cache_read_args *a, void *stream) {
+  SIG3D_REQUIRE(a != nullptr, "no arguments");
+  if (int e = check_cache("sig3d_cache_read", a->dtype, a->b, a->capacity, a->hkv, a->d)) return e;
+  SIG3D_REQUIRE(a->n >= 1 && a->n <= a->capacity && (long)a->n * a->d < (1l << 33), "row count out of range");
+  SIG3D_REQUIRE(a->k_cache && a->v_cache && a->lengths && a->k_out && a->v_out, "missing array");
+  SIG3D_REQUIRE((a->k_scale == nullptr) == (a->v_scale == nullptr), "k_scale and v_scale come together");
+  SIG3D_REQUIRE(aligned16(a->k_cache) && aligned16(a->v_cache) && aligned16(a->k_out) && aligned16(a->v_out),
+                "addresses must be 16-byte aligned");
+  const ReadParams p = {a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->lengths, a->k_out, a->v_out, a->n, a->capacity, a->hkv};
+  const dim3 grid(sig3d_ceil_div((long)a->n * (a->d / 8), 256), a->hkv, a->b);
+  return by_type(a->dtype, a->d, [&](auto t, auto dd) {
     typedef decltype(t) T;
     constexpr int D = decltype(dd)::value;
-    if (k_scale) cache_read_kernel<T, D, true><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+    if (a->k_scale) cache_read_kernel<T, D, true><<<grid, 256, 0, (hipStream_t)stream>>>(p);
     else cache_read_kernel<T, D, false><<<grid, 256, 0, (hipStream_t)stream>>>(p);
     SIG3D_LAUNCH_CHECK("cache_read_kernel");
     return 0;

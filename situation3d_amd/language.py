@@ -63,33 +63,49 @@ def _bucket_struct(buckets, max_distance, bidirectional):
     return s
 
 
-def _dense_rows(t):
-    """(tensor, its strides but the innermost) with rows as the kernels read them: dense, 16-byte aligned; copied if not."""
-    for _ in range(2):
-        e = t.element_size()
-        strides = [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
-        if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in strides) and strides[1] * e < 1 << 24:
-            return t, strides
-        t = t.clone(memory_format=torch.contiguous_format)
-    raise RuntimeError("could not lay out a tensor of shape %s" % (tuple(t.shape),))
+def _readable(shape, stride, itemsize):
+    """Rows as the kernels read them: dense, strides multiples of 16 bytes, a token's below 16 MB."""
+    return (stride[-1] == 1 or shape[-1] == 1) and all(n == 1 or s >= 0 and s * itemsize % 16 == 0 for n, s in
+                                                      zip(shape[:-1], stride[:-1])) and stride[1] * itemsize < 1 << 24
 
 
-def _check_heads(q, k, v, what):
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+def _strides(shape, stride):
+    return [0 if n == 1 else s for n, s in zip(shape[:-1], stride[:-1])]
+
+
+def _rows(t):
+    """`t`, or a dense copy where the kernels cannot read its rows (differentiable)."""
+    if t.data_ptr() % 16 == 0 and _readable(t.shape, t.stride(), t.element_size()):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _launch(name, args, device):
+    """One library call on the current stream of `device`."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _check_heads(q, k, v, dtypes, what):
+    if len(q) != 4 or len(k) != 4 or len(v) != 4:
         raise RuntimeError("%s takes (batch, tokens, heads, head size) tensors" % what)
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    if dtypes[0] not in _DTYPES or len(set(dtypes)) != 1:
         raise RuntimeError("%s: q, k, v must share one of float32, bfloat16, float16" % what)
-    if q.shape[3] not in _HEAD_SIZES:
-        raise RuntimeError("%s: head size %d, the HIP kernels are built for 64, 96 and 128" % (what, q.shape[3]))
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise RuntimeError("%s: q %s, k %s, v %s do not belong together" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise RuntimeError("%s: %d heads over %d key heads" % (what, q.shape[2], k.shape[2]))
+    if q[3] not in _HEAD_SIZES:
+        raise RuntimeError("%s: head size %d, the HIP kernels are built for 64, 96 and 128" % (what, q[3]))
+    if k != v or k[0] != q[0] or k[3] != q[3]:
+        raise RuntimeError("%s: q %s, k %s, v %s do not belong together" % (what, tuple(q), tuple(k), tuple(v)))
+    if k[2] == 0 or q[2] % k[2]:
+        raise RuntimeError("%s: %d heads over %d key heads" % (what, q[2], k[2]))
 
 
-def _check_table(table, q, what):
-    if table is not None and (table.dim() != 2 or table.shape[1] != q.shape[2] or table.dtype != q.dtype):
-        raise RuntimeError("%s: the bias table is (buckets, heads) = (., %d) in q's type" % (what, q.shape[2]))
+def _check_table(shape, dtype, heads, q_dtype, what):
+    if shape is not None and (len(shape) != 2 or shape[1] != heads or dtype != q_dtype):
+        raise RuntimeError("%s: the bias table is (buckets, heads) = (., %d) in q's type" % (what, heads))
 
 
 def _int_array(t, shape, device, name):
@@ -118,70 +134,96 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _rel_args(q, k, v, table, cfg, arrays, out, out32, lse, grad=None, grads=(None,) * 4, work=None):
+@functools.lru_cache(maxsize=1024)
+def _rel_template(q, qs, k, ks, v, vs, dtypes, table, table_dtype, cfg):
+    """Everything about a call that shapes, strides and types decide, checked once: the argument struct without its addresses,
+    and whether q, k, v can be read as they are."""
+    _check_heads(q, k, v, dtypes, "relative_attention")
+    _check_table(table, table_dtype, q[2], dtypes[0], "relative_attention")
     scale, bidirectional, max_distance, causal, offset = cfg
-    q, qs = _dense_rows(q)
-    k, ks = _dense_rows(k)
-    v, vs = _dense_rows(v)
-    gs = [0, 0, 0]
-    if grad is not None:
-        grad, gs = _dense_rows(grad)
-    b, nq, h, d = q.shape
-    rows = 0 if table is None else table.shape[0]
-    a = _lib.RelAttentionArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(table), *[_ptr(x) for x in arrays], _ptr(out), _ptr(out32), _ptr(lse),
-        _ptr(grad), *[_ptr(x) for x in grads], _ptr(work), *qs, *ks, *vs, *gs, _DTYPES[q.dtype], b, nq, k.shape[1], h, k.shape[2], d,
-        int(causal), offset, rows, scale, _bucket_struct(rows, max_distance, bidirectional))
-    return a, (q, k, v, grad)                  # copies that the strides belong to live until the launch
+    rows = 0 if table is None else table[0]
+    e = dtypes[0].itemsize
+    a = _lib.RelAttentionArgs(dtype=_DTYPES[dtypes[0]], b=q[0], nq=q[1], nk=k[1], h=q[2], hkv=k[2], d=q[3], causal=int(causal),
+                              query_offset=offset, table_rows=rows, scale=scale,
+                              buckets=_bucket_struct(rows, max_distance, bidirectional))
+    for name, shape, stride in (("q", q, qs), ("k", k, ks), ("v", v, vs)):
+        for dim, s in zip("bnh", _strides(shape, stride)):
+            setattr(a, "%s_%s" % (name, dim), s)
+    return a, all(_readable(*x, e) for x in ((q, qs), (k, ks), (v, vs)))
 
 
-def _rel_forward(q, k, v, table, cfg, arrays, keep):
+def _rel_args(q, k, v, table, cfg, arrays):
+    """(argument struct, readable): see _rel_template."""
+    a, ok = _rel_template(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), (q.dtype, k.dtype, v.dtype),
+                          None if table is None else table.shape, None if table is None else table.dtype, cfg)
+    a = _lib.RelAttentionArgs.from_buffer_copy(a)
+    a.q, a.k, a.v = qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if table is not None:
+        a.table = table.data_ptr()
+    lengths, prefix, ranges = arrays
+    if lengths is not None:
+        a.key_lengths = lengths.data_ptr()
+    if prefix is not None:
+        a.prefix_lengths = prefix.data_ptr()
+    if ranges is not None:
+        a.key_ranges = ranges.data_ptr()
+    return a, ok and not (qp | kp | vp) & 15
+
+
+def _rel_forward(a, q, k, keep):
+    b, nq, h, d = shape = q.shape
     dev = q.device
-    b, nq, h, d = q.shape
-    out = torch.empty((b, nq, h, d), dtype=q.dtype, device=dev)
+    out = torch.empty(shape, dtype=q.dtype, device=dev)
     # the unrounded output: delta = dO.O decides dS where one key has almost all of a row, and O rounded to 8 bits would not do
-    out32 = torch.empty((b, nq, h, d), dtype=torch.float32, device=dev) if keep else None
+    out32 = torch.empty(shape, dtype=torch.float32, device=dev) if keep else None
     lse = torch.empty((b, h, nq), dtype=torch.float32, device=dev) if keep else None
     if out.numel() == 0:
         return out, out32, lse
     if k.shape[1] == 0:
         return out.zero_(), out32.zero_() if keep else None, lse
-    a, held = _rel_args(q, k, v, table, cfg, arrays, out, out32, lse)
-    with torch.cuda.device(dev):
-        _lib.call("sig3d_rel_attention_fwd", ctypes.byref(a), _lib.stream_ptr(dev))
-    del held
+    a.out = out.data_ptr()
+    if keep:
+        a.out32, a.lse = out32.data_ptr(), lse.data_ptr()
+    _launch("sig3d_rel_attention_fwd", ctypes.byref(a), dev)
     return out, out32, lse
 
 
 class _RelativeAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, cfg, arrays):
-        out, out32, lse = _rel_forward(q, k, v, table, cfg, arrays, True)
-        ctx.save_for_backward(q, k, v, table, out, out32, lse, *arrays)
+    def forward(ctx, q, k, v, table, cfg, arrays, a):
+        out, out32, lse = _rel_forward(a, q, k, True)
+        ctx.save_for_backward(q, k, v, table, out32, lse, *arrays)
         ctx.cfg = cfg
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, table, out, out32, lse, *arrays = ctx.saved_tensors
-        dev = q.device
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk, dv = torch.empty(k.shape, dtype=k.dtype, device=dev), torch.empty(v.shape, dtype=v.dtype, device=dev)
-        dtable = None if table is None else torch.empty_like(table, memory_format=torch.contiguous_format)
+        q, k, v, table, out32, lse, *arrays = ctx.saved_tensors
+        dev, dtype = q.device, q.dtype
+        dq = torch.empty(q.shape, dtype=dtype, device=dev)
+        dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
+        dtable = None if table is None else torch.empty(table.shape, dtype=dtype, device=dev)
         if q.numel() == 0 or k.numel() == 0:
             for t in (dq, dk, dv, dtable):
                 if t is not None:
                     t.zero_()
-            return dq, dk, dv, dtable, None, None
-        # the query layout of `out` is dense: it names the strides, the kernels read out32
-        a, held = _rel_args(q, k, v, table, ctx.cfg, arrays, out, out32, lse, grad, (dq, dk, dv, dtable))
-        work = torch.empty(_lib.load().sig3d_rel_attention_bwd_work_floats(ctypes.byref(a)), dtype=torch.float32, device=dev)
+            return dq, dk, dv, dtable, None, None, None
+        a, ok = _rel_args(q, k, v, table, ctx.cfg, arrays)
+        if not ok:                               # saved tensors came back laid out differently (hooks)
+            q, k, v = _rows(q), _rows(k), _rows(v)
+            a, _ = _rel_args(q, k, v, table, ctx.cfg, arrays)
+        grad = _rows(grad)
+        a.grad_b, a.grad_n, a.grad_h = _strides(grad.shape, grad.stride())
+        # (out is not read again: the kernels take the unrounded copy; its address only has to be one)
+        a.out, a.out32, a.lse, a.grad = out32.data_ptr(), out32.data_ptr(), lse.data_ptr(), grad.data_ptr()
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        if dtable is not None:
+            a.dtable = dtable.data_ptr()
+        work = torch.empty(_lib.load().sig3d_rel_attention_bwd_work_floats(a), dtype=torch.float32, device=dev)
         a.work = work.data_ptr()
-        with torch.cuda.device(dev):
-            _lib.call("sig3d_rel_attention_bwd", ctypes.byref(a), _lib.stream_ptr(dev))
-        del held
-        return dq, dk, dv, dtable, None, None
+        _launch("sig3d_rel_attention_bwd", ctypes.byref(a), dev)
+        return dq, dk, dv, dtable, None, None, None
 
 
 def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, max_distance=128, causal=False, query_offset=0,
@@ -199,24 +241,29 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
       must be finite for the others.
     -> (b, nq, h, d) in q's type."""
     dev = _lib.require_device(q, k, v, table, key_lengths, prefix_lengths, key_ranges)
-    _check_heads(q, k, v, "relative_attention")
-    _check_table(table, q, "relative_attention")
     if prefix_lengths is not None and not causal:
         raise RuntimeError("relative_attention: prefix_lengths only means something with causal=True")
-    b, nq = q.shape[:2]
-    arrays = (_int_array(key_lengths, (b,), dev, "key_lengths"), _int_array(prefix_lengths, (b,), dev, "prefix_lengths"),
-              _int_array(key_ranges, (b, nq, 2), dev, "key_ranges"))
-    cfg = (float(q.shape[3] ** -0.5 if scale is None else scale), bool(bidirectional), int(max_distance), bool(causal),
+    cfg = (float(q.shape[-1] ** -0.5 if scale is None else scale), bool(bidirectional), int(max_distance), bool(causal),
            int(query_offset))
     if not math.isfinite(cfg[0]):
         raise RuntimeError("relative_attention: scale must be finite")
     if table is not None:
-        _bucket_struct(table.shape[0], cfg[2], cfg[1])         # refuses here, not inside backward
         table = table.contiguous()
+    none = (None, None, None)
+    a, ok = _rel_args(q, k, v, table, cfg, none)
+    b, nq = q.shape[:2]
+    arrays = none
+    if key_lengths is not None or prefix_lengths is not None or key_ranges is not None:
+        arrays = (_int_array(key_lengths, (b,), dev, "key_lengths"), _int_array(prefix_lengths, (b,), dev, "prefix_lengths"),
+                  _int_array(key_ranges, (b, nq, 2), dev, "key_ranges"))
+        a.key_lengths, a.prefix_lengths, a.key_ranges = (None if x is None else x.data_ptr() for x in arrays)
+    if not ok:
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        a, _ = _rel_args(q, k, v, table, cfg, arrays)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or table is not None and table.requires_grad):
-        return _RelativeAttentionFn.apply(q, k, v, table, cfg, arrays)
-    return _rel_forward(q, k, v, table, cfg, arrays, False)[0]
+        return _RelativeAttentionFn.apply(q, k, v, table, cfg, arrays, a)
+    return _rel_forward(a, q, k, False)[0]
 
 
 class KVCache:
@@ -253,8 +300,8 @@ class KVCache:
         """Tokens k, v (batch, t, kv_heads, head_dim) in the cache's type: the first counts[b] (None: t) go to rows
         start[b] + i (None: behind what is there), and lengths[b] becomes start[b] + counts[b]; both int32 (batch,).  Tokens
         beyond the capacity are dropped and lengths stops there; other rows stay as they are."""
-        dev = _lib.require_device(k, v, self.lengths, start, counts)
-        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != self.batch or tuple(k.shape[2:]) != (self.kv_heads, self.head_dim):
+        dev = _lib.require_device(self.lengths, k, v, start, counts)
+        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != self.batch or k.shape[2] != self.kv_heads or k.shape[3] != self.head_dim:
             raise RuntimeError("KVCache.append: k and v must be (%d, t, %d, %d)" % (self.batch, self.kv_heads, self.head_dim))
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise RuntimeError("KVCache.append: the cache takes %s" % self.dtype)
@@ -264,13 +311,12 @@ class KVCache:
             if start is not None:
                 self.lengths.copy_(start.clamp(0, self.capacity))
             return
-        k, ks = _dense_rows(k.detach())
-        v, vs = _dense_rows(v.detach())
+        k, v = _rows(k), _rows(v)
         a = _lib.CacheAppendArgs(k.data_ptr(), v.data_ptr(), self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs),
-                                 _ptr(start), _ptr(counts), self.lengths.data_ptr(), *ks, *vs, _DTYPES[self.dtype], self.batch, t,
-                                 self.capacity, self.kv_heads, self.head_dim)
-        with torch.cuda.device(dev):
-            _lib.call("sig3d_cache_append", ctypes.byref(a), _lib.stream_ptr(dev))
+                                 _ptr(start), _ptr(counts), self.lengths.data_ptr(), *_strides(k.shape, k.stride()),
+                                 *_strides(v.shape, v.stride()), _DTYPES[self.dtype], self.batch, t, self.capacity, self.kv_heads,
+                                 self.head_dim)
+        _launch("sig3d_cache_append", ctypes.byref(a), dev)
 
     def read(self, tokens=None):
         """(k, v) (batch, tokens, kv_heads, head_dim) in the cache's type: the values that the first `tokens` rows (None: all)
@@ -278,12 +324,13 @@ class KVCache:
         n = self.capacity if tokens is None else int(tokens)
         if not 0 <= n <= self.capacity:
             raise RuntimeError("KVCache.read: %d of %d rows" % (n, self.capacity))
-        k, v = (torch.empty((self.batch, n, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device) for _ in range(2))
+        shape = (self.batch, n, self.kv_heads, self.head_dim)
+        k, v = torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device)
         if n:
-            with torch.cuda.device(self.device):
-                _lib.call("sig3d_cache_read", _DTYPES[self.dtype], self.batch, n, self.capacity, self.kv_heads, self.head_dim,
-                          self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs), self.lengths.data_ptr(),
-                          k.data_ptr(), v.data_ptr(), _lib.stream_ptr(self.device))
+            a = _lib.CacheReadArgs(self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs), self.lengths.data_ptr(),
+                                   k.data_ptr(), v.data_ptr(), _DTYPES[self.dtype], self.batch, n, self.capacity, self.kv_heads,
+                                   self.head_dim)
+            _launch("sig3d_cache_read", ctypes.byref(a), self.device)
         return k, v
 
 
@@ -301,32 +348,59 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
     what = "decode_attention"
     if q.dim() != 4 or q.dtype != cache.dtype:
         raise RuntimeError("%s: q is (batch, new tokens, heads, head size) in the cache's type" % what)
-    b, t, h, d = q.shape
+    b, t, h, d = shape = q.shape
     if b != cache.batch or d != cache.head_dim or h == 0 or h % cache.kv_heads:
         raise RuntimeError("%s: q %s does not belong to a cache of %d sequences, %d heads of %d" % (
-            what, tuple(q.shape), cache.batch, cache.kv_heads, cache.head_dim))
+            what, tuple(shape), cache.batch, cache.kv_heads, cache.head_dim))
     if shared is not None and (shared.dtype != cache.dtype or shared.quantized != cache.quantized or shared.kv_heads != cache.kv_heads
                                or shared.head_dim != d or b % shared.batch):
         raise RuntimeError("%s: the shared sequences must be held like the cache's, their number dividing %d" % (what, b))
-    _check_table(table, q, what)
-    counts = _int_array(counts, (b,), dev, "counts")
-    q, qs = _dense_rows(q.detach())
-    out = torch.empty((b, t, h, d), dtype=q.dtype, device=dev)
-    if t == 0:
-        return out
     rows = 0
     if table is not None:
-        table, rows = table.detach().contiguous(), table.shape[0]
-    s = shared
-    a = _lib.DecodeAttentionArgs(
-        q.data_ptr(), _ptr(table), cache._k.data_ptr(), cache._v.data_ptr(), _ptr(s and s._k), _ptr(s and s._v), _ptr(cache._ks),
-        _ptr(cache._vs), _ptr(s and s._ks), _ptr(s and s._vs), cache.lengths.data_ptr(), _ptr(s and s.lengths), _ptr(counts),
-        out.data_ptr(), None, *qs, _DTYPES[q.dtype], b, t, h, cache.kv_heads, d, cache.capacity, s.batch if s else 0,
-        s.capacity if s else 0, rows, float(d ** -0.5 if scale is None else scale), _bucket_struct(rows, max_distance, bool(bidirectional)))
-    need = _lib.load().sig3d_decode_attention_work_floats(ctypes.byref(a))
+        _check_table(table.shape, table.dtype, h, q.dtype, what)
+        table, rows = table.contiguous(), table.shape[0]
+    if counts is not None:
+        counts = _int_array(counts, (b,), dev, "counts")
+    out = torch.empty(shape, dtype=q.dtype, device=dev)
+    if t == 0:
+        return out
+    q = _rows(q)
+    a, need = _decode_template(shape, q.stride(), _DTYPES[q.dtype], cache.kv_heads, cache.capacity, cache.quantized,
+                               shared.batch if shared is not None else 0, shared.capacity if shared is not None else 0, rows,
+                               float(d ** -0.5 if scale is None else scale), int(max_distance), bool(bidirectional))
+    a = _lib.DecodeAttentionArgs.from_buffer_copy(a)
+    a.q, a.out, a.k_cache, a.v_cache = q.data_ptr(), out.data_ptr(), cache._k.data_ptr(), cache._v.data_ptr()
+    a.lengths = cache.lengths.data_ptr()
+    if cache.quantized:
+        a.k_scale, a.v_scale = cache._ks.data_ptr(), cache._vs.data_ptr()
+    if shared is not None:
+        a.shared_k, a.shared_v, a.shared_lengths = shared._k.data_ptr(), shared._v.data_ptr(), shared.lengths.data_ptr()
+        if cache.quantized:
+            a.shared_k_scale, a.shared_v_scale = shared._ks.data_ptr(), shared._vs.data_ptr()
+    if rows:
+        a.table = table.data_ptr()
+    if counts is not None:
+        a.counts = counts.data_ptr()
     if need:
         work = torch.empty(need, dtype=torch.float32, device=dev)
         a.work = work.data_ptr()
-    with torch.cuda.device(dev):
-        _lib.call("sig3d_decode_attention", ctypes.byref(a), _lib.stream_ptr(dev))
+    _launch("sig3d_decode_attention", ctypes.byref(a), dev)
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_template(q, qs, dtype, hkv, capacity, quantized, groups, shared_capacity, rows, scale, max_distance, bidirectional):
+    """What shapes and types decide of a decode_attention call: its argument struct without addresses, its workspace."""
+    if not math.isfinite(scale):
+        raise RuntimeError("decode_attention: scale must be finite")
+    b, t, h, d = q
+    a = _lib.DecodeAttentionArgs(dtype=dtype, b=b, t=t, h=h, hkv=hkv, d=d, capacity=capacity, groups=groups,
+                                 shared_capacity=shared_capacity, table_rows=rows, scale=scale,
+                                 buckets=_bucket_struct(rows, max_distance, bidirectional))
+    a.q_b, a.q_n, a.q_h = _strides(q, qs)
+    a.table = 16 if rows else None                    # the size does not depend on the address, only on there being one
+    need = _lib.load().sig3d_decode_attention_work_floats(a)
+    if need < 0:
+        raise RuntimeError("decode_attention: " + _lib.load().sig3d_last_error().decode())
+    a.table = None
+    return a, need

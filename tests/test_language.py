@@ -52,7 +52,7 @@ def test_document_ranges():
 def test_language_structs_match_the_c_header(tmp_path):
     from situation3d_amd import _lib
     structs = {"sig3d_rel_buckets": _lib.RelBuckets, "sig3d_rel_attention_args": _lib.RelAttentionArgs,
-               "sig3d_cache_append_args": _lib.CacheAppendArgs, "sig3d_decode_attention_args": _lib.DecodeAttentionArgs}
+               "sig3d_cache_append_args": _lib.CacheAppendArgs, "sig3d_cache_read_args": _lib.CacheReadArgs, "sig3d_decode_attention_args": _lib.DecodeAttentionArgs}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "sig3d_hip.h"', 'int main(void) {',
              'printf("max %d %d\\n", SIG3D_REL_MAX_BUCKETS, SIG3D_REL_MAX_REACH);']
     for name, cls in structs.items():
@@ -120,7 +120,7 @@ def test_rel_attention_bwd_refuses(bad):
 def test_null_arguments_are_refused():
     from situation3d_amd import _lib
     lib = _lib.load()
-    for name in ("sig3d_rel_attention_fwd", "sig3d_rel_attention_bwd", "sig3d_cache_append", "sig3d_decode_attention"):
+    for name in ("sig3d_rel_attention_fwd", "sig3d_rel_attention_bwd", "sig3d_cache_append", "sig3d_cache_read", "sig3d_decode_attention"):
         with pytest.raises(_lib.Sig3dError):
             _lib.call(name, None, None)
     assert lib.sig3d_rel_attention_bwd_work_floats(None) == -1 and lib.sig3d_decode_attention_work_floats(None) == -1
@@ -137,13 +137,13 @@ def test_cache_append_refuses(bad):
         _lib.call("sig3d_cache_append", ctypes.byref(_lib.CacheAppendArgs(**{**base, **bad})), None)
 
 
-@pytest.mark.parametrize("at,value", [(0, 3), (1, 0), (2, 0), (2, 9), (3, 0), (4, 0), (5, 65), (6, None), (8, None), (10, None), (11, A + 4)])
-def test_cache_read_refuses(at, value):
+@pytest.mark.parametrize("bad", [dict(dtype=3), dict(b=0), dict(n=0), dict(n=9), dict(capacity=0), dict(hkv=0), dict(d=65), dict(k_cache=0),
+                                 dict(k_scale=0), dict(v_scale=0), dict(lengths=0), dict(k_out=0), dict(k_out=A + 4)], ids=str)
+def test_cache_read_refuses(bad):
     from situation3d_amd import _lib
-    args = [1, 1, 4, 8, 1, 64, A, A, A, A, A, A, A, None]
-    args[at] = value
+    base = dict(k_cache=A, v_cache=A, k_scale=A, v_scale=A, lengths=A, k_out=A, v_out=A, dtype=1, b=1, n=4, capacity=8, hkv=1, d=64)
     with pytest.raises(_lib.Sig3dError):
-        _lib.call("sig3d_cache_read", *args)
+        _lib.call("sig3d_cache_read", ctypes.byref(_lib.CacheReadArgs(**{**base, **bad})), None)
 
 
 DECODE_BAD = [dict(dtype=4), dict(b=0), dict(t=0), dict(h=3), dict(hkv=0), dict(d=32), dict(capacity=0), dict(groups=3), dict(groups=-1),
