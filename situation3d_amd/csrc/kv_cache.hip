@@ -23,84 +23,99 @@ struct AppendParams {
   int t, capacity, hkv;
 };
 
-// Four lanes hold a row, lane l the 16-byte pieces l, l + 4, ...
-template <typename T, int D> struct Row {
-  static constexpr int PER = 16 / (int)sizeof(T), N = D / PER / 4;
+// LANES neighbouring lanes hold a row, one 16-byte piece each (of 96 elements: 12 of 16 lanes, 24 of 32): a load instruction
+// moves whole rows.  (Four lanes with every fourth piece: 64 bytes of a row at a time, 72 us for 8192 x 4 x 8 rows of 128
+// floats instead of 70, and as much for the read: 72 instead of 46.)
+template <typename T, int D> struct Piece {
+  static constexpr int PER = 16 / (int)sizeof(T), USED = D / PER, LANES = USED <= 8 ? 8 : USED <= 16 ? 16 : 32;
   typedef T piece __attribute__((ext_vector_type(PER)));
-  piece x[N];
-  __device__ __forceinline__ void load(const T *row, int l) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const piece *>(row + (l + 4 * i) * PER);
-  }
-  __device__ __forceinline__ void put(T *row, int l) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<piece *>(row + (l + 4 * i) * PER) = x[i];
-  }
-  // the scale's exponent: infinities and NaN do not count
-  __device__ __forceinline__ int exponent() const {
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const float a = fabsf((float)x[i][e]);
-        top = a < INFINITY ? fmaxf(top, a) : top;
-      }
+  static __device__ __forceinline__ float over_lanes(float top) {
     top = fmaxf(top, __builtin_bit_cast(float, dpp_i32<0xB1>(__builtin_bit_cast(int, top))));
     top = fmaxf(top, __builtin_bit_cast(float, dpp_i32<0x4E>(__builtin_bit_cast(int, top))));
+    top = fmaxf(top, __builtin_bit_cast(float, dpp_i32<0x141>(__builtin_bit_cast(int, top))));
+    if constexpr (LANES >= 16) top = fmaxf(top, __builtin_bit_cast(float, dpp_i32<0x140>(__builtin_bit_cast(int, top))));
+    if constexpr (LANES == 32) top = fmaxf(top, __shfl_xor(top, 16));
+    return top;
+  }
+  // A row's e4m3 values, and its scale by its first lane.  Infinities and NaN do not count in the scale; infinities, which only
+  // a wave that has one looks for, become the largest value.
+  static __device__ __forceinline__ void quantize(unsigned char *to, float *scale, piece x, bool mine, bool first) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) top = fmaxf(top, fabsf((float)x[e]));        // fmaxf drops NaN
+    top = over_lanes(top);
+    const bool infinite = __any(top == INFINITY);
+    if (infinite) {
+      top = 0.f;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const float a = fabsf((float)x[e]);
+        top = a < INFINITY ? fmaxf(top, a) : top;
+      }
+      top = over_lanes(top);
+    }
     // top = m 2^x with m in [0.5, 1), 448 = 0.875 2^9; scales stay normal numbers
     const int ex = __builtin_amdgcn_frexp_expf(top) - 9 + (__builtin_amdgcn_frexp_mantf(top) > 0.875f ? 1 : 0);
-    return top > 0.f ? max(ex, -126) : 0;
-  }
-  __device__ __forceinline__ void put_e4m3(unsigned char *row, int l, int exponent) const {
+    const int exponent = top > 0.f ? max(ex, -126) : 0;
     const float inv = __builtin_ldexpf(1.f, -exponent);
+    float y[PER];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      unsigned w[PER / 4];
+    for (int e = 0; e < PER; ++e) y[e] = (float)x[e] * inv;
+    if (infinite) {
 #pragma unroll
-      for (int g = 0; g < PER / 4; ++g) {
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[e] = (float)x[i][4 * g + e] * inv;
-          y[e] = fabsf(y[e]) > 448.f ? copysignf(448.f, y[e]) : y[e];      // infinities; NaN stays
-        }
-        int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-        p = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], p, true);
-        w[g] = (unsigned)p;
-      }
-      unsigned *to = reinterpret_cast<unsigned *>(row + (l + 4 * i) * PER);
-      if constexpr (PER == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[PER / 4 - 1]);
-      else to[0] = w[0];
+      for (int e = 0; e < PER; ++e) y[e] = fabsf(y[e]) > 448.f ? copysignf(448.f, y[e]) : y[e];
     }
+    unsigned w[PER / 4];
+#pragma unroll
+    for (int g = 0; g < PER / 4; ++g) {
+      const int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * g], y[4 * g + 1], 0, false);
+      w[g] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * g + 2], y[4 * g + 3], p, true);
+    }
+    if (mine) {
+      if constexpr (PER == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[PER / 4 - 1]);
+      else *reinterpret_cast<unsigned *>(to) = w[0];
+    }
+    if (first) *scale = __builtin_ldexpf(1.f, exponent);
   }
 };
+
+// Rows a thread has in flight.  Reads wait on memory (3000 cycles a request at 3.5 TB/s in total); 1, 2 and 4 rows, tokens before
+// heads and heads before tokens all measured within 10 %.
+constexpr int UNROLL = 2;
 
 // grid (blocks of rows, b).  One block a sequence, or `start` given: lengths is updated here, after everyone has read it.
 template <typename T, int D, bool Q>
 __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p) {
-  const int b = blockIdx.y, l = threadIdx.x & 3, rows = p.hkv * p.t;
+  typedef Piece<T, D> P;
+  constexpr int ROWS = 256 / P::LANES;
+  const int b = blockIdx.y, l = threadIdx.x % P::LANES, rows = p.hkv * p.t;
   const int first = p.start ? p.start[b] : p.lengths[b];
   const int count = p.counts ? min(max(p.counts[b], 0), p.t) : p.t;
-  for (int r = blockIdx.x * 64 + (threadIdx.x >> 2); r < rows; r += gridDim.x * 64) {
-    const int head = r / p.t, i = r - head * p.t;
-    const long to = (long)first + i;
-    if (i >= count || to < 0 || to >= p.capacity) continue;        // the four lanes of a row agree
-    Row<T, D> k, v;
-    k.load(reinterpret_cast<const T *>(p.k) + b * p.k_b + i * p.k_n + head * p.k_h, l);
-    v.load(reinterpret_cast<const T *>(p.v) + b * p.v_b + i * p.v_n + head * p.v_h, l);
-    const long row = ((long)b * p.hkv + head) * p.capacity + to;
-    if constexpr (Q) {
-      const int ek = k.exponent(), ev = v.exponent();
-      k.put_e4m3(reinterpret_cast<unsigned char *>(p.k_cache) + row * D, l, ek);
-      v.put_e4m3(reinterpret_cast<unsigned char *>(p.v_cache) + row * D, l, ev);
-      if (l == 0) {
-        p.k_scale[row] = __builtin_ldexpf(1.f, ek);
-        p.v_scale[row] = __builtin_ldexpf(1.f, ev);
+  const bool mine = P::USED == P::LANES || l < P::USED;
+  for (int r0 = blockIdx.x * ROWS * UNROLL + threadIdx.x / P::LANES; r0 < rows; r0 += gridDim.x * ROWS * UNROLL) {
+    typename P::piece k[UNROLL], v[UNROLL];
+    long row[UNROLL];                                              // of the cache; negative: nothing to do (a row's lanes agree)
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int r = min(r0 + u * ROWS, rows - 1), head = r / p.t, i = r - head * p.t;
+      const long to = (long)first + i;
+      row[u] = r0 + u * ROWS < rows && i < count && to >= 0 && to < p.capacity ? ((long)b * p.hkv + head) * p.capacity + to : -1;
+      // no condition on a load (it would be waited for inside): what is not to be moved repeats the last token that is
+      const int from = min(i, max(count - 1, 0)), e = min(l, P::USED - 1) * P::PER;
+      k[u] = *reinterpret_cast<const typename P::piece *>(reinterpret_cast<const T *>(p.k) + b * p.k_b + from * p.k_n + head * p.k_h + e);
+      v[u] = *reinterpret_cast<const typename P::piece *>(reinterpret_cast<const T *>(p.v) + b * p.v_b + from * p.v_n + head * p.v_h + e);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (row[u] < 0) continue;
+      const long at = row[u] * D + l * P::PER;
+      if constexpr (Q) {
+        P::quantize(reinterpret_cast<unsigned char *>(p.k_cache) + at, p.k_scale + row[u], k[u], mine, l == 0);
+        P::quantize(reinterpret_cast<unsigned char *>(p.v_cache) + at, p.v_scale + row[u], v[u], mine, l == 0);
+      } else if (mine) {
+        *reinterpret_cast<typename P::piece *>(reinterpret_cast<T *>(p.k_cache) + at) = k[u];
+        *reinterpret_cast<typename P::piece *>(reinterpret_cast<T *>(p.v_cache) + at) = v[u];
       }
-    } else {
-      k.put(reinterpret_cast<T *>(p.k_cache) + row * D, l);
-      v.put(reinterpret_cast<T *>(p.v_cache) + row * D, l);
     }
   }
   if (gridDim.x == 1 || p.start) {
@@ -124,28 +139,36 @@ struct ReadParams {
   int n, capacity, hkv;
 };
 
-// a thread: eight elements of a K row and of the V row beside it.  grid (n * D / 8 / 256, hkv, b)
+// a thread: 16 bytes of a K row of the result and of the V row beside it.  grid (pieces / 256, hkv, b)
 template <typename T, int D, bool Q>
 __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
-  const int c = blockIdx.x * 256 + threadIdx.x, i = c / (D / 8), o = c - i * (D / 8);
+  typedef Piece<T, D> P;
+  typedef typename P::piece piece;
+  const int c = blockIdx.x * 256 + threadIdx.x, i = c / P::USED, o = c - i * P::USED;
   if (i >= p.n) return;
   const int b = blockIdx.z, head = blockIdx.y;
-  frag_t<T> k{}, v{};
+  piece k{}, v{};
   if (i < p.lengths[b]) {
-    const long row = ((long)b * p.hkv + head) * p.capacity + i;
+    const long row = ((long)b * p.hkv + head) * p.capacity + i, at = row * D + o * P::PER;
     if constexpr (Q) {
-      const uint2 wk = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(p.k) + row * D + 8 * o);
-      const uint2 wv = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned char *>(p.v) + row * D + 8 * o);
-      k = from_e4m3<T>(wk, p.k_scale[row]);
-      v = from_e4m3<T>(wv, p.v_scale[row]);
+      const unsigned *kp = reinterpret_cast<const unsigned *>(reinterpret_cast<const unsigned char *>(p.k) + at);
+      const unsigned *vp = reinterpret_cast<const unsigned *>(reinterpret_cast<const unsigned char *>(p.v) + at);
+      const float ks = p.k_scale[row], vs = p.v_scale[row];
+      if constexpr (P::PER == 8) {
+        k = from_e4m3<T>(*reinterpret_cast<const uint2 *>(kp), ks);
+        v = from_e4m3<T>(*reinterpret_cast<const uint2 *>(vp), vs);
+      } else {
+        k = __builtin_shufflevector(from_e4m3<T>(make_uint2(*kp, 0), ks), f32x8{}, 0, 1, 2, 3);
+        v = __builtin_shufflevector(from_e4m3<T>(make_uint2(*vp, 0), vs), f32x8{}, 0, 1, 2, 3);
+      }
     } else {
-      k = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.k) + row * D + 8 * o);
-      v = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.v) + row * D + 8 * o);
+      k = *reinterpret_cast<const piece *>(reinterpret_cast<const T *>(p.k) + at);
+      v = *reinterpret_cast<const piece *>(reinterpret_cast<const T *>(p.v) + at);
     }
   }
-  const long to = (((long)b * p.n + i) * p.hkv + head) * D + 8 * o;
-  *reinterpret_cast<frag_t<T> *>(reinterpret_cast<T *>(p.k_out) + to) = k;
-  *reinterpret_cast<frag_t<T> *>(reinterpret_cast<T *>(p.v_out) + to) = v;
+  const long to = (((long)b * p.n + i) * p.hkv + head) * D + o * P::PER;
+  *reinterpret_cast<piece *>(reinterpret_cast<T *>(p.k_out) + to) = k;
+  *reinterpret_cast<piece *>(reinterpret_cast<T *>(p.v_out) + to) = v;
 }
 
 int check_cache(const char *where, int dtype, int b, int capacity, int hkv, int d) {
@@ -174,7 +197,8 @@ extern "C" int sig3d_cache_append(const sig3d_cache_append_args *a, void *stream
   // without `start` every workgroup of a sequence reads the length that the call moves: one workgroup up to 512 rows (a
   // decoding step: 32 heads are half a pass), else a launch of its own moves it
   const bool one = !a->start && rows <= 512;
-  const dim3 grid(one ? 1 : sig3d_ceil_div(rows, 64), a->b);
+  const int piece = a->dtype == 0 ? 4 : 8, lanes = a->d / piece <= 8 ? 8 : a->d / piece <= 16 ? 16 : 32;
+  const dim3 grid(one ? 1 : sig3d_ceil_div(rows, 256 / lanes * UNROLL), a->b);
   const int err = by_type(a->dtype, a->d, [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
@@ -198,7 +222,7 @@ extern "C" int sig3d_cache_read(const sig3d_cache_read_args *a, void *stream) {
   SIG3D_REQUIRE(aligned16(a->k_cache) && aligned16(a->v_cache) && aligned16(a->k_out) && aligned16(a->v_out),
                 "addresses must be 16-byte aligned");
   const ReadParams p = {a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->lengths, a->k_out, a->v_out, a->n, a->capacity, a->hkv};
-  const dim3 grid(sig3d_ceil_div((long)a->n * (a->d / 8), 256), a->hkv, a->b);
+  const dim3 grid(sig3d_ceil_div((long)a->n * (a->d / (a->dtype == 0 ? 4 : 8)), 256), a->hkv, a->b);
   return by_type(a->dtype, a->d, [&](auto t, auto dd) {
     typedef decltype(t) T;
     constexpr int D = decltype(dd)::value;
