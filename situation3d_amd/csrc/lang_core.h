@@ -83,6 +83,9 @@ __device__ __forceinline__ float sum_halves(float x) {
   both_halves(x, lo, hi);
   return lo + hi;
 }
+// Waits for every load so far.  Before a loop: what was loaded ahead of it would else be waited for inside, by counts that also
+// cover the loads which that iteration has just sent out.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt 0, the others free
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ int wave_min_i32(int v) { return -wave_allreduce_max_i32(-v); }
 __device__ __forceinline__ int wave_max_i32(int v) { return wave_allreduce_max_i32(v); }

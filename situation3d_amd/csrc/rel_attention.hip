@@ -203,6 +203,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
   __syncthreads();
   const bool biased = p.bk.n > 0;
   const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
+  loads_done();
   int buf = 0;
   for (int t = first; t < whi; t += KT, buf ^= 1) {
     const bool more = t + KT < whi;
@@ -403,6 +404,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void r
   float behind = 0.f, ahead = 0.f;
   __syncthreads();
   const float bias_behind = biased ? bias[0] : 0.f, bias_ahead = biased ? bias[2 * (reach + EDGE)] : 0.f;
+  loads_done();
   int buf = 0;
   for (int t = first; t < whi; t += KT, buf ^= 1) {
     const bool more = t + KT < whi;
@@ -649,6 +651,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void re
         put(0, todo[0] & ~(1 << 30));
       }
       __syncthreads();
+      loads_done();
       for (int i = 0; i < n; ++i) {
         const int buf = i & 1, entry = todo[i], q0 = (entry & ~(1 << 30)) * QT;
         const bool cut = entry >> 30;
