@@ -130,6 +130,8 @@ constexpr float SLACK = 8.f;                  // of the forward pass's reference
 constexpr int P_UP = 8, DS_UP = 3;            // f16: exponents that P and dS are raised by (see the top)
 
 template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+// keys of a tile of the dQ kernel: 32 leave LDS and registers for two workgroups a CU where a row is long
+template <typename T> constexpr int dq_tile(int d) { return sizeof(T) == 2 && d == 64 ? 64 : 32; }
 
 // s (scaled scores of a 32 x 32 block, in log2 units) += bias.  first = position of register 0's row minus that of the lane's
 // column, i.e. register r stands at relative position first + sign * (16 (r >> 3) + (r & 7)).
@@ -315,9 +317,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
 // address and mask instructions and twice the LDS time: 88 us instead of DQ_US for 4 x 32 heads of 432 tokens.)
 constexpr int DIAG_ROW = 36, DIAG = 64 * DIAG_ROW;        // floats; 36: 16-byte rows whose columns spread over the banks
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 || D == 128 ? 1 : 2) void rel_bwd_dq_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
-  constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
+  constexpr int KT = dq_tile<T>(D), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
   extern __shared__ __align__(16) char lds[];
   float *bias = reinterpret_cast<float *>(lds + 4 * TB);
   const int reach = p.bk.reach, span = bias_floats(reach);
@@ -821,9 +823,10 @@ template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream)
   static sig3d_once_per_device once_q, once_kv;
   const int span = (bias_floats(p.bk.reach) + 3) / 4 * 4;
   const size_t tiles = 4 * key_tile<T>() * Tile<T, D>::ROW;
+  const size_t dq_tiles = 4 * dq_tile<T>(D) * Tile<T, D>::ROW;
   if (int e = allow_lds(rel_bwd_dq_kernel<T, D, NW>, once_q)) return e;
   if (int e = allow_lds(rel_bwd_dkv_kernel<T, D, NW>, once_kv)) return e;
-  rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, tiles + ((NW + 1) * span + NW * DIAG) * sizeof(float), stream>>>(p);
+  rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, dq_tiles + ((NW + 1) * span + NW * DIAG) * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dq_kernel");
   rel_bwd_dkv_kernel<T, D, NW><<<p.b * p.hkv * p.ktiles * p.head_splits * p.query_splits, NW * 64, tiles + span * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dkv_kernel");
