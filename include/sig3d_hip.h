@@ -882,7 +882,7 @@ typedef struct {
                                                  sum of exponentials, +inf where a query sees no key */
   const void *grad;                           /* backward: d out */
   void *dq, *dk, *dv, *dtable;                /* backward: dense, of dtype; dtable NULL without a bias */
-  float *work;                                /* backward: sig3d_rel_attention_bwd_work_floats() floats */
+  float *work;                                /* sig3d_rel_attention_{fwd,bwd}_work_floats() floats; may be NULL where that is 0 */
   long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, grad_b, grad_n, grad_h;
   int dtype, b, nq, nk, h, hkv, d, causal, query_offset, table_rows;
   float scale;
@@ -890,6 +890,7 @@ typedef struct {
 } sig3d_rel_attention_args;
 int sig3d_rel_attention_fwd(const sig3d_rel_attention_args *args, void *stream);
 int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *args, void *stream);
+long sig3d_rel_attention_fwd_work_floats(const sig3d_rel_attention_args *args);
 long sig3d_rel_attention_bwd_work_floats(const sig3d_rel_attention_args *args);
 
 /* A cache of b sequences: k_cache / v_cache (b, hkv, capacity, d), of dtype, or e4m3 (OCP, 1 byte) with one f32 scale per

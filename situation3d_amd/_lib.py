@@ -346,7 +346,8 @@ def bq_levels_workspace_bytes(batch, arr):
 
 INFO_SYMBOLS = ("sig3d_version", "sig3d_last_error", "sig3d_voxelize_workspace_bytes", "sig3d_fps_blocks_workspace_bytes",
                 "sig3d_ball_query_levels_workspace_bytes", "sig3d_pooled_heads_work_floats",
-                "sig3d_mlp_layer_dw_stream_work_floats", "sig3d_gemmp_work_floats", "sig3d_rel_attention_bwd_work_floats",
+                "sig3d_mlp_layer_dw_stream_work_floats", "sig3d_gemmp_work_floats", "sig3d_rel_attention_fwd_work_floats",
+                "sig3d_rel_attention_bwd_work_floats",
                 "sig3d_decode_attention_work_floats")
 
 _lib = None
@@ -383,6 +384,8 @@ def load():
     lib.sig3d_pooled_heads_work_floats.restype = ctypes.c_long
     lib.sig3d_mlp_layer_dw_stream_work_floats.argtypes = [_I, _I, _I, ctypes.c_long]
     lib.sig3d_mlp_layer_dw_stream_work_floats.restype = ctypes.c_long
+    lib.sig3d_rel_attention_fwd_work_floats.argtypes = [ctypes.POINTER(RelAttentionArgs)]
+    lib.sig3d_rel_attention_fwd_work_floats.restype = ctypes.c_long
     lib.sig3d_rel_attention_bwd_work_floats.argtypes = [ctypes.POINTER(RelAttentionArgs)]
     lib.sig3d_rel_attention_bwd_work_floats.restype = ctypes.c_long
     lib.sig3d_decode_attention_work_floats.argtypes = [ctypes.POINTER(DecodeAttentionArgs)]

@@ -31,10 +31,11 @@ struct Params {
   void *out, *dq, *dk, *dv, *dtable;
   float *out32, *lse, *delta, *hist;
   float *part;                                // backward: dK, dV of every split, (2, splits, b, nk, hkv, d), or NULL: one split
+  float *piece, *piece_ml;                    // one output, maximum and sum (forward), one dQ for every key split, or NULL
   int4 *blocks;                               // backward: interval summary of every 32 queries
   int *tops;                                  // backward, f16: exponent of the largest |dO| of a head's 32 queries
   long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, grad_b, grad_n, grad_h;
-  int b, nq, nk, h, hkv, group, causal, offset, table_rows, qtiles, ktiles, head_splits, query_splits;
+  int b, nq, nk, h, hkv, group, causal, offset, table_rows, qtiles, ktiles, head_splits, query_splits, key_splits;
   float scale;
   Buckets bk;
 };
@@ -66,6 +67,15 @@ __device__ __forceinline__ Span span_of(int lo, int hi, bool valid) {
   s.all_lo = wave_max_i32(valid ? lo : 0);
   s.all_hi = wave_min_i32(valid ? hi : INT_MAX);
   return s;
+}
+
+// [lo, hi) -> its part `split` of `splits`, in whole tiles
+template <int KT> __device__ __forceinline__ void cut_piece(int &lo, int &hi, int split, int splits) {
+  if (lo >= hi) return;
+  const int first = lo / KT, tiles = (hi + KT - 1) / KT - first, share = (tiles + splits - 1) / splits;
+  lo = max(lo, (first + split * share) * KT);
+  hi = min(hi, (first + (split + 1) * share) * KT);
+  if (lo >= hi) hi = 0;                        // nothing left: the loop over [lo, hi) starts at 0
 }
 
 // Consecutive workgroups go to the 8 XCDs in turn; give each XCD a contiguous share of the work instead, so that the
@@ -162,7 +172,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;      // causal: the long rows first
+  const int split = id % p.key_splits, item = id / p.key_splits;
+  const int bh = item / p.qtiles, qt = p.qtiles - 1 - item % p.qtiles;      // causal: the long rows first
   const int b = bh / p.h, head = bh - b * p.h;
   BiasFill<T> fill;
   fill.start(p.bk, p.table, p.h, head, tid);
@@ -182,6 +193,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
     wlo = min(wlo, ends[0][w]);
     whi = max(whi, ends[1][w]);
   }
+  if (p.key_splits > 1) cut_piece<KT>(wlo, whi, split, p.key_splits);
   const int kvh = head / p.group;
   const T *kb = reinterpret_cast<const T *>(p.k) + b * p.k_b + kvh * p.k_h;
   const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
@@ -300,10 +312,50 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void
   const bool empty = lo >= hi;
   const float inv = empty ? 0.f : 1.f / l;
   const long row = (((long)b * p.nq + qi) * p.h + head) * D;
+  if (p.piece) {
+    store_row<float, D>(p.piece + split * ((long)p.b * p.nq * p.h * D) + row, o, 1.f, half);
+    if (half == 0)
+      reinterpret_cast<float2 *>(p.piece_ml)[(split * (long)p.b * p.h + bh) * p.nq + qi] = make_float2(m, l);
+    return;
+  }
   store_row<T, D>(reinterpret_cast<T *>(p.out) + row, o, inv, half);
   if (p.out32) {
     store_row<float, D>(p.out32 + row, o, inv, half);
     if (half == 0) p.lse[((long)b * p.h + head) * p.nq + qi] = empty ? INFINITY : m + __builtin_amdgcn_logf(l);
+  }
+}
+
+// Joins the key splits of a row in their order: D / 4 lanes a row (query, head).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void rel_join_kernel(const Params p) {
+  constexpr int PER = D / 4, ROWS = 256 / PER;
+  const int e = threadIdx.x % PER;
+  const long row = (long)blockIdx.x * ROWS + threadIdx.x / PER, rows = (long)p.b * p.nq * p.h;      // (b, nq, h)
+  if (threadIdx.x / PER >= ROWS || row >= rows) return;
+  const int head = (int)(row % p.h);
+  const long at = row / p.h, stat = (at / p.nq * p.h + head) * p.nq + at % p.nq;                    // (b, h, nq)
+  const float2 *ml = reinterpret_cast<const float2 *>(p.piece_ml) + stat;
+  float top = -INFINITY, sum = 0.f;
+  for (int s = 0; s < p.key_splits; ++s) top = fmaxf(top, ml[s * rows].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 x = {};
+#pragma unroll 4
+  for (int s = 0; s < p.key_splits; ++s) {
+    const float2 v = ml[s * rows];
+    const float keep = exp2_(v.x - base);
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(p.piece + (s * rows + row) * D + 4 * e);
+    sum = __builtin_fmaf(v.y, keep, sum);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(y[q], keep, x[q]);
+  }
+  const bool empty = top == -INFINITY && sum == 0.f;
+  const float inv = empty ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) x[q] *= inv;
+  reinterpret_cast<vec4_t<T> *>(p.out)[row * PER + e] = to_vec4<T>(x);
+  if (p.out32) {
+    reinterpret_cast<f32x4 *>(p.out32)[row * PER + e] = x;
+    if (e == 0) p.lse[stat] = empty ? INFINITY : top + __builtin_amdgcn_logf(sum);
   }
 }
 
@@ -328,7 +380,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bh = id / p.qtiles, qt = p.qtiles - 1 - id % p.qtiles;
+  const int split = id % p.key_splits, item = id / p.key_splits;
+  const int bh = item / p.qtiles, qt = p.qtiles - 1 - item % p.qtiles;
   const int b = bh / p.h, head = bh - b * p.h;
   BiasFill<T> fill;
   fill.start(p.bk, p.table, p.h, head, tid);
@@ -340,7 +393,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
   if (lane == 0) {
     ends[0][wave] = sp.any_lo;
     ends[1][wave] = sp.any_hi;
-    if (head == 0) p.blocks[((long)b * p.qtiles + qt) * NW + wave] = make_int4(sp.any_lo, sp.any_hi, sp.all_lo, sp.all_hi);
+    if (head == 0 && split == 0) p.blocks[((long)b * p.qtiles + qt) * NW + wave] = make_int4(sp.any_lo, sp.any_hi, sp.all_lo, sp.all_hi);
   }
   __syncthreads();
   int wlo = INT_MAX, whi = 0;
@@ -349,6 +402,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
     wlo = min(wlo, ends[0][w]);
     whi = max(whi, ends[1][w]);
   }
+  if (p.key_splits > 1) cut_piece<KT>(wlo, whi, split, p.key_splits);
   const int kvh = head / p.group;
   const T *kb = reinterpret_cast<const T *>(p.k) + b * p.k_b + kvh * p.k_h;
   const T *vb = reinterpret_cast<const T *>(p.v) + b * p.v_b + kvh * p.v_h;
@@ -372,7 +426,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
   }
   delta = sum_halves(delta);
   if (!valid) lse = INFINITY;
-  if (valid && half == 0) p.delta[stat] = delta;
+  if (valid && half == 0 && split == 0) p.delta[stat] = delta;
   float undo = 1.f;                                       // dS is held times 1 / undo
   if constexpr (narrow<T>()) {
     float top = 0.f;
@@ -386,7 +440,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
     undo = __builtin_ldexpf(1.f, e - DS_UP);
     lse += (float)(e - DS_UP);
     const int most = wave_max_i32(plain ? -64 : e);
-    if (lane == 0) p.tops[((long)bh * p.qtiles + qt) * NW + wave] = most;
+    if (lane == 0 && split == 0) p.tops[((long)bh * p.qtiles + qt) * NW + wave] = most;
   }
   const bool biased = p.bk.n > 0;
   if (biased) {
@@ -483,7 +537,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
     }
     __syncthreads();
   }
-  if (valid) store_row<T, D>(reinterpret_cast<T *>(p.dq) + row, dq, p.scale * undo, half);
+  if (valid) {
+    if (p.piece) store_row<float, D>(p.piece + split * ((long)p.b * p.nq * p.h * D) + row, dq, p.scale * undo, half);
+    else store_row<T, D>(reinterpret_cast<T *>(p.dq) + row, dq, p.scale * undo, half);
+  }
   if (!biased) return;
   const float far_behind = wave_allreduce_sum_f32(behind), far_ahead = wave_allreduce_sum_f32(ahead);
   if (lane == 0) {
@@ -493,7 +550,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
   __syncthreads();
   // distances -> buckets (keys ahead share bucket 0 unless they have their own), one row of partial sums a workgroup: the
   // waves' rows are added first, then a wave takes every fourth bucket, its lanes the distances
-  float *part = p.hist + ((long)bh * p.qtiles + qt) * p.table_rows;
+  float *part = p.hist + (((long)bh * p.qtiles + qt) * p.key_splits + split) * p.table_rows;
   const int pitch = (span + 3) / 4 * 4, most = reach + EDGE;
   for (int i = tid; i < span; i += NT) {
     float x = sums[i];
@@ -757,7 +814,7 @@ int check(const char *where, const sig3d_rel_attention_args *a) {
        "q, k, v, out must be 16-byte aligned addresses");
   LANG_NEED(where, (a->out32 == nullptr) == (a->lse == nullptr) && aligned16(a->out32), "out32 and lse come together");
   if (int e = check_buckets(where, a->buckets, a->table, a->table_rows)) return e;
-  LANG_NEED(where, (long)a->b * a->h * ((a->nq + 31) / 32) < INT_MAX && (long)a->b * a->h * ((a->nk + 31) / 32) < INT_MAX / 16, "grid too large");
+  LANG_NEED(where, (long)a->b * a->h * ((a->nq + 31) / 32) < INT_MAX / 16 && (long)a->b * a->h * ((a->nk + 31) / 32) < INT_MAX / 16, "grid too large");
   return 0;
 }
 
@@ -778,6 +835,8 @@ Params params(const sig3d_rel_attention_args *a) {
   return p;
 }
 
+int key_splits(const sig3d_rel_attention_args *a);
+
 // workspace of the backward pass: delta (b h nq), interval summaries (b, 4 per 128 queries) int4, exponents of |dO| (f16),
 // partial table gradients
 long work_delta(const sig3d_rel_attention_args *a) { return ((long)a->b * a->h * a->nq + 3) / 4 * 4; }
@@ -786,7 +845,24 @@ long work_tops(const sig3d_rel_attention_args *a) {
   return a->dtype == 2 ? ((long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * NW + 3) / 4 * 4 : 0;
 }
 long work_hist(const sig3d_rel_attention_args *a) {
-  return a->buckets.n > 0 ? (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * a->table_rows : 0;
+  return a->buckets.n > 0 ? (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * key_splits(a) * a->table_rows : 0;
+}
+
+// Key splits of the forward and the dQ kernel: where batch, heads and tiles of 128 queries are fewer workgroups than two for each
+// of 256 CUs, down to 8 tiles of keys (f32: 4; a tile there is 6000 cycles of the matrix cores).  (2 x 1021 tokens, 8 heads of 96
+// floats: 126 us forward and 176 us dQ as 128 workgroups.)
+int key_splits(const sig3d_rel_attention_args *a) {
+  const long items = (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32);
+  const int tiles = sig3d_ceil_div(a->nk, a->dtype == 0 ? 32 : 64), least = a->dtype == 0 ? 4 : 8;
+  return (int)std::max<long>(1, std::min<long>(std::min<long>(16, (512 + items - 1) / items), tiles / least));
+}
+long work_piece(const sig3d_rel_attention_args *a) {
+  const int n = key_splits(a);
+  return n > 1 ? (long)n * a->b * a->nq * a->h * a->d : 0;
+}
+long work_ml(const sig3d_rel_attention_args *a) {
+  const int n = key_splits(a);
+  return n > 1 ? ((long)n * a->b * a->nq * a->h * 2 + 3) / 4 * 4 : 0;
 }
 
 // Splits of the dK / dV kernel.  Causal and packed rows make workgroups very unequal -- the first keys of a document are seen by
@@ -814,8 +890,12 @@ template <typename T, int D> int launch_fwd(const Params &p, hipStream_t stream)
   static sig3d_once_per_device once;
   const size_t lds = 4 * key_tile<T>() * Tile<T, D>::ROW + bias_floats(p.bk.reach) * sizeof(float);
   if (int e = allow_lds(rel_fwd_kernel<T, D, NW>, once)) return e;
-  rel_fwd_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, lds, stream>>>(p);
+  rel_fwd_kernel<T, D, NW><<<p.b * p.h * p.qtiles * p.key_splits, NW * 64, lds, stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_fwd_kernel");
+  if (p.piece) {
+    rel_join_kernel<T, D><<<sig3d_ceil_div((long)p.b * p.nq * p.h, 256 / (D / 4)), 256, 0, stream>>>(p);
+    SIG3D_LAUNCH_CHECK("rel_join_kernel");
+  }
   return 0;
 }
 
@@ -826,8 +906,14 @@ template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream)
   const size_t dq_tiles = 4 * dq_tile<T>(D) * Tile<T, D>::ROW;
   if (int e = allow_lds(rel_bwd_dq_kernel<T, D, NW>, once_q)) return e;
   if (int e = allow_lds(rel_bwd_dkv_kernel<T, D, NW>, once_kv)) return e;
-  rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles, NW * 64, dq_tiles + ((NW + 1) * span + NW * DIAG) * sizeof(float), stream>>>(p);
+  rel_bwd_dq_kernel<T, D, NW><<<p.b * p.h * p.qtiles * p.key_splits, NW * 64, dq_tiles + ((NW + 1) * span + NW * DIAG) * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dq_kernel");
+  if (p.piece) {
+    const long quads = (long)p.b * p.nq * p.h * D / 4;
+    rel_bwd_fold_kernel<T><<<dim3(sig3d_ceil_div(quads, 256), 1), 256, 0, stream>>>(p.piece, p.key_splits, quads,
+                                                                                   reinterpret_cast<T *>(p.dq), nullptr);
+    SIG3D_LAUNCH_CHECK("rel_bwd_fold_kernel");
+  }
   rel_bwd_dkv_kernel<T, D, NW><<<p.b * p.hkv * p.ktiles * p.head_splits * p.query_splits, NW * 64, tiles + span * sizeof(float), stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_bwd_dkv_kernel");
   if (p.part) {
@@ -838,7 +924,7 @@ template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream)
   }
   if (p.bk.n > 0) {
     rel_bwd_table_kernel<T><<<dim3(p.h, sig3d_ceil_div(p.table_rows, 4)), 256, 0, stream>>>(
-        p.hist, p.b, p.h, p.qtiles, p.table_rows, reinterpret_cast<T *>(p.dtable));
+        p.hist, p.b, p.h, p.qtiles * p.key_splits, p.table_rows, reinterpret_cast<T *>(p.dtable));
     SIG3D_LAUNCH_CHECK("rel_bwd_table_kernel");
   }
   return 0;
@@ -848,15 +934,26 @@ template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream)
 
 extern "C" int sig3d_rel_attention_fwd(const sig3d_rel_attention_args *a, void *stream) {
   if (int e = check("sig3d_rel_attention_fwd", a)) return e;
-  const Params p = params(a);
+  Params p = params(a);
+  p.key_splits = key_splits(a);
+  if (p.key_splits > 1) {
+    SIG3D_REQUIRE(a->work && aligned16(a->work), "missing workspace");
+    p.piece = a->work;
+    p.piece_ml = a->work + work_piece(a);
+  }
   return by_type(a->dtype, a->d, [&](auto t, auto d) {
     return launch_fwd<decltype(t), decltype(d)::value>(p, (hipStream_t)stream);
   });
 }
 
+extern "C" long sig3d_rel_attention_fwd_work_floats(const sig3d_rel_attention_args *a) {
+  if (check("sig3d_rel_attention_fwd_work_floats", a)) return -1;
+  return work_piece(a) + work_ml(a);
+}
+
 extern "C" long sig3d_rel_attention_bwd_work_floats(const sig3d_rel_attention_args *a) {
   if (check("sig3d_rel_attention_bwd_work_floats", a)) return -1;
-  return work_delta(a) + work_blocks(a) + work_tops(a) + (work_hist(a) + 3) / 4 * 4 + work_part(a);
+  return work_delta(a) + work_blocks(a) + work_tops(a) + (work_hist(a) + 3) / 4 * 4 + work_part(a) + work_piece(a);
 }
 
 extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *stream) {
@@ -878,6 +975,8 @@ extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *
   p.head_splits = s.heads;
   p.query_splits = s.queries;
   if (s.heads * s.queries > 1) p.part = p.hist + (work_hist(a) + 3) / 4 * 4;
+  p.key_splits = key_splits(a);
+  if (p.key_splits > 1) p.piece = p.hist + (work_hist(a) + 3) / 4 * 4 + work_part(a);
   return by_type(a->dtype, a->d, [&](auto t, auto d) {
     return launch_bwd<decltype(t), decltype(d)::value>(p, (hipStream_t)stream);
   });

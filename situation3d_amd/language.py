@@ -137,7 +137,7 @@ def _ptr(t):
 @functools.lru_cache(maxsize=1024)
 def _rel_template(q, qs, k, ks, v, vs, dtypes, table, table_dtype, cfg):
     """Everything about a call that shapes, strides and types decide, checked once: the argument struct without its addresses,
-    and whether q, k, v can be read as they are."""
+    whether q, k, v can be read as they are, and the floats of workspace forward and backward."""
     _check_heads(q, k, v, dtypes, "relative_attention")
     _check_table(table, table_dtype, q[2], dtypes[0], "relative_attention")
     scale, bidirectional, max_distance, causal, offset = cfg
@@ -149,12 +149,20 @@ def _rel_template(q, qs, k, ks, v, vs, dtypes, table, table_dtype, cfg):
     for name, shape, stride in (("q", q, qs), ("k", k, ks), ("v", v, vs)):
         for dim, s in zip("bnh", _strides(shape, stride)):
             setattr(a, "%s_%s" % (name, dim), s)
-    return a, all(_readable(*x, e) for x in ((q, qs), (k, ks), (v, vs)))
+    ok = all(_readable(*x, e) for x in ((q, qs), (k, ks), (v, vs)))
+    work = (0, 0)
+    if ok and q[0] and q[1] and k[1]:
+        a.q = a.k = a.v = a.out = a.table = 16           # the sizes do not depend on addresses, only on there being some
+        work = tuple(f(a) for f in (_lib.load().sig3d_rel_attention_fwd_work_floats, _lib.load().sig3d_rel_attention_bwd_work_floats))
+        if min(work) < 0:
+            raise RuntimeError("relative_attention: " + _lib.load().sig3d_last_error().decode())
+        a.q = a.k = a.v = a.out = a.table = None
+    return a, ok, work
 
 
 def _rel_args(q, k, v, table, cfg, arrays):
-    """(argument struct, readable): see _rel_template."""
-    a, ok = _rel_template(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), (q.dtype, k.dtype, v.dtype),
+    """(argument struct, readable, workspaces): see _rel_template."""
+    a, ok, work = _rel_template(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), (q.dtype, k.dtype, v.dtype),
                           None if table is None else table.shape, None if table is None else table.dtype, cfg)
     a = _lib.RelAttentionArgs.from_buffer_copy(a)
     a.q, a.k, a.v = qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
@@ -167,10 +175,10 @@ def _rel_args(q, k, v, table, cfg, arrays):
         a.prefix_lengths = prefix.data_ptr()
     if ranges is not None:
         a.key_ranges = ranges.data_ptr()
-    return a, ok and not (qp | kp | vp) & 15
+    return a, ok and not (qp | kp | vp) & 15, work
 
 
-def _rel_forward(a, q, k, keep):
+def _rel_forward(a, q, k, keep, need):
     b, nq, h, d = shape = q.shape
     dev = q.device
     out = torch.empty(shape, dtype=q.dtype, device=dev)
@@ -182,6 +190,9 @@ def _rel_forward(a, q, k, keep):
     if k.shape[1] == 0:
         return out.zero_(), out32.zero_() if keep else None, lse
     a.out = out.data_ptr()
+    if need:
+        work = torch.empty(need, dtype=torch.float32, device=dev)
+        a.work = work.data_ptr()
     if keep:
         a.out32, a.lse = out32.data_ptr(), lse.data_ptr()
     _launch("sig3d_rel_attention_fwd", ctypes.byref(a), dev)
@@ -190,8 +201,8 @@ def _rel_forward(a, q, k, keep):
 
 class _RelativeAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, cfg, arrays, a):
-        out, out32, lse = _rel_forward(a, q, k, True)
+    def forward(ctx, q, k, v, table, cfg, arrays, a, need):
+        out, out32, lse = _rel_forward(a, q, k, True, need)
         ctx.save_for_backward(q, k, v, table, out32, lse, *arrays)
         ctx.cfg = cfg
         return out
@@ -208,11 +219,11 @@ class _RelativeAttentionFn(torch.autograd.Function):
             for t in (dq, dk, dv, dtable):
                 if t is not None:
                     t.zero_()
-            return dq, dk, dv, dtable, None, None, None
-        a, ok = _rel_args(q, k, v, table, ctx.cfg, arrays)
+            return dq, dk, dv, dtable, None, None, None, None
+        a, ok, work = _rel_args(q, k, v, table, ctx.cfg, arrays)
         if not ok:                               # saved tensors came back laid out differently (hooks)
             q, k, v = _rows(q), _rows(k), _rows(v)
-            a, _ = _rel_args(q, k, v, table, ctx.cfg, arrays)
+            a, _, work = _rel_args(q, k, v, table, ctx.cfg, arrays)
         grad = _rows(grad)
         a.grad_b, a.grad_n, a.grad_h = _strides(grad.shape, grad.stride())
         # (out is not read again: the kernels take the unrounded copy; its address only has to be one)
@@ -220,10 +231,10 @@ class _RelativeAttentionFn(torch.autograd.Function):
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if dtable is not None:
             a.dtable = dtable.data_ptr()
-        work = torch.empty(_lib.load().sig3d_rel_attention_bwd_work_floats(a), dtype=torch.float32, device=dev)
+        work = torch.empty(work[1], dtype=torch.float32, device=dev)
         a.work = work.data_ptr()
         _launch("sig3d_rel_attention_bwd", ctypes.byref(a), dev)
-        return dq, dk, dv, dtable, None, None, None
+        return dq, dk, dv, dtable, None, None, None, None
 
 
 def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, max_distance=128, causal=False, query_offset=0,
@@ -250,7 +261,7 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
     if table is not None:
         table = table.contiguous()
     none = (None, None, None)
-    a, ok = _rel_args(q, k, v, table, cfg, none)
+    a, ok, work = _rel_args(q, k, v, table, cfg, none)
     b, nq = q.shape[:2]
     arrays = none
     if key_lengths is not None or prefix_lengths is not None or key_ranges is not None:
@@ -259,11 +270,11 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
         a.key_lengths, a.prefix_lengths, a.key_ranges = (None if x is None else x.data_ptr() for x in arrays)
     if not ok:
         q, k, v = _rows(q), _rows(k), _rows(v)
-        a, _ = _rel_args(q, k, v, table, cfg, arrays)
+        a, _, work = _rel_args(q, k, v, table, cfg, arrays)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or table is not None and table.requires_grad):
-        return _RelativeAttentionFn.apply(q, k, v, table, cfg, arrays, a)
-    return _rel_forward(a, q, k, False)[0]
+        return _RelativeAttentionFn.apply(q, k, v, table, cfg, arrays, a, work[0])
+    return _rel_forward(a, q, k, False, work[0])[0]
 
 
 class KVCache:

@@ -107,6 +107,16 @@ def test_rel_attention_refuses(n, name):
     with pytest.raises(_lib.Sig3dError):
         _lib.call(name, ctypes.byref(a), None)
     assert _lib.load().sig3d_rel_attention_bwd_work_floats(ctypes.byref(a)) == -1
+    assert _lib.load().sig3d_rel_attention_fwd_work_floats(ctypes.byref(a)) == -1
+
+
+def test_rel_attention_fwd_wants_its_workspace():
+    from situation3d_amd import _lib
+    a = _rel_args(nq=32, nk=4096, work=0)
+    assert _lib.load().sig3d_rel_attention_fwd_work_floats(ctypes.byref(a)) > 0
+    with pytest.raises(_lib.Sig3dError):
+        _lib.call("sig3d_rel_attention_fwd", ctypes.byref(a), None)
+    assert _lib.load().sig3d_rel_attention_fwd_work_floats(ctypes.byref(_rel_args())) == 0
 
 
 @pytest.mark.parametrize("bad", [dict(grad=0), dict(dq=0), dict(dk=0), dict(dv=0), dict(work=0), dict(dtable=0), dict(out32=0, lse=0),
