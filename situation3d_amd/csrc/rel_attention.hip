@@ -163,7 +163,7 @@ __device__ __forceinline__ Where where(int k0, int n, int p0, int reach) {
 // the next tile's loads are in flight while the current one is used, one barrier a tile.
 // S^T = K Q^T, then O^T = V^T P^T: a query is one lane (and lane ^ 32), its softmax is in-lane work.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void rel_fwd_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? (D == 128 ? 1 : 2) : D == 64 ? 3 : 2) void rel_fwd_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
   extern __shared__ __align__(16) char lds[];
