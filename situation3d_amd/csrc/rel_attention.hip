@@ -142,6 +142,8 @@ constexpr int P_UP = 8, DS_UP = 3;            // f16: exponents that P and dS ar
 template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
 // keys of a tile of the dQ kernel: 32 leave LDS and registers for two workgroups a CU where a row is long
 template <typename T> constexpr int dq_tile(int d) { return sizeof(T) == 2 && d == 64 ? 64 : 32; }
+// queries of a tile of the dK / dV kernel, likewise (at 128 wide K, V and both sums fill a SIMD with one wave anyway)
+template <typename T> constexpr int dkv_tile(int d) { return sizeof(T) == 2 && d != 96 ? 64 : 32; }
 
 // s (scaled scores of a 32 x 32 block, in log2 units) += bias.  first = position of register 0's row minus that of the lane's
 // column, i.e. register r stands at relative position first + sign * (16 (r >> 3) + (r & 7)).
@@ -600,9 +602,9 @@ __global__ __launch_bounds__(256) void rel_bwd_table_kernel(const float *hist, i
 // there are too few workgroups for the chip (see splits_of): then heads and runs of queries become workgroups of their own,
 // which leave f32 sums that a small kernel adds in order.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D == 64 ? 2 : 1) void rel_bwd_dkv_kernel(const Params p) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D < 128 ? 2 : 1) void rel_bwd_dkv_kernel(const Params p) {
   typedef Tile<T, D> TL;
-  constexpr int QT = key_tile<T>(), NT = NW * 64, SUB = QT / 32, TB = QT * TL::ROW;
+  constexpr int QT = dkv_tile<T>(D), NT = NW * 64, SUB = QT / 32, TB = QT * TL::ROW;
   extern __shared__ __align__(16) char lds[];
   __shared__ float stats[2][2][QT];            // [buffer][lse, delta]
   __shared__ int rows[2][2][QT];               // [buffer][lo, hi]
@@ -876,7 +878,7 @@ Splits splits_of(const sig3d_rel_attention_args *a) {
   Splits s = {1, 1};
   for (int n = 2; n <= want; ++n)
     if (group % n == 0) s.heads = n;
-  const int tiles = sig3d_ceil_div(a->nq, a->dtype == 0 ? 32 : 64);
+  const int tiles = sig3d_ceil_div(a->nq, a->dtype == 0 || a->d == 96 ? 32 : 64);
   s.queries = std::max(1, std::min(want / s.heads, tiles / 8));
   return s;
 }
@@ -902,7 +904,7 @@ template <typename T, int D> int launch_fwd(const Params &p, hipStream_t stream)
 template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream) {
   static sig3d_once_per_device once_q, once_kv;
   const int span = (bias_floats(p.bk.reach) + 3) / 4 * 4;
-  const size_t tiles = 4 * key_tile<T>() * Tile<T, D>::ROW;
+  const size_t tiles = 4 * dkv_tile<T>(D) * Tile<T, D>::ROW;
   const size_t dq_tiles = 4 * dq_tile<T>(D) * Tile<T, D>::ROW;
   if (int e = allow_lds(rel_bwd_dq_kernel<T, D, NW>, once_q)) return e;
   if (int e = allow_lds(rel_bwd_dkv_kernel<T, D, NW>, once_kv)) return e;
