@@ -529,13 +529,16 @@ Plan plan(const sig3d_decode_attention_args *a) {
   s.joined = each > 0 && (each == 1 || a->shared_capacity <= 256);
   s.nb = 1;
   const int own_rows = a->capacity + (s.joined ? a->shared_capacity : 0);
-  s.own_splits = (int)std::min<long>(std::max<long>(1, 4096 / base), sig3d_ceil_div(own_rows, LEAST * KT));
+  // About four workgroups of own rows for every CU (more pieces: more starts and joins; 8 ragged contexts of up to 30 000 rows took
+  // 79 us with 4096 workgroups, 72 with 1024), and one of shared rows: they are the long ones, and what a workgroup costs before
+  // and after its tiles is spread over more of them (2 scenes, 48 questions: 75 us with 768, 60 with 256).
+  s.own_splits = (int)std::min<long>(std::max<long>(1, 1024 / base), sig3d_ceil_div(own_rows, LEAST * KT));
   if (each > 0 && !s.joined) {
     const long rows = (long)each * per;
     s.nb = rows > 16 ? BLOCKS : 1;
     s.shared_tiles = sig3d_ceil_div(rows, 16 * s.nb);
     const long far = (long)a->groups * a->hkv * s.shared_tiles;
-    s.shared_splits = (int)std::min<long>(std::max<long>(1, 768 / far), sig3d_ceil_div(a->shared_capacity, LEAST * KT));
+    s.shared_splits = (int)std::min<long>(std::max<long>(1, 256 / far), sig3d_ceil_div(a->shared_capacity, LEAST * KT));
     s.shared_items = (int)(far * s.shared_splits);
   }
   s.own_items = (int)(base * s.own_splits);
