@@ -895,14 +895,15 @@ long sig3d_rel_attention_bwd_work_floats(const sig3d_rel_attention_args *args);
 
 /* A cache of b sequences: k_cache / v_cache (b, hkv, capacity, d), of dtype, or e4m3 (OCP, 1 byte) with one f32 scale per
  * row, k_scale / v_scale (b, hkv, capacity): the smallest power of two with max |row| <= 448 scale, values rounded to
- * nearest even; infinite values are held as +-448 scale and do not count in the maximum, NaN stays NaN. */
+ * nearest even, and to at most the largest value of 4 significant bits that dtype holds; infinite values are held as the
+ * largest value (+-448 scale where dtype has that) and do not count in the maximum, NaN stays NaN. */
 typedef struct {
   const void *k, *v;                          /* (b, t, hkv, d): new tokens */
   void *k_cache, *v_cache;
   float *k_scale, *v_scale;                   /* NULL: the cache is of dtype */
   const int *start, *counts;                  /* (b) or NULL: token i < counts[b] (default t) goes to row start[b] + i (default
                                                  lengths[b] + i); rows outside [0, capacity) are dropped */
-  int *lengths;                               /* (b): set to start + counts, at most capacity */
+  int *lengths;                               /* (b): set to start + counts, at most capacity; start and counts lie elsewhere */
   long k_b, k_n, k_h, v_b, v_n, v_h;
   int dtype, b, t, capacity, hkv, d;
 } sig3d_cache_append_args;

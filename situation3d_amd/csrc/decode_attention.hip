@@ -2,7 +2,7 @@
 //
 // Sequence i sees [the rows of shared sequence i / (b / groups) | its own rows up to the query].  Decoding is bound by reading
 // keys and values, so each part is read as few times as its users allow: the queries of ALL sequences of a group that share a
-// key head are rows of one product over the shared keys (up to 64 rows a workgroup), and only the own rows are read per
+// key head are rows of one product over the shared keys (up to 32 rows a workgroup), and only the own rows are read per
 // sequence.  Both parts are cut along the keys until the chip is full; a piece leaves (max, sum, unnormalised output), and a
 // second kernel joins the pieces of a row in their order.  Small calls -- one piece, nothing worth sharing -- are one launch:
 // a workgroup walks shared and own rows of one sequence and writes the result itself.
@@ -132,7 +132,7 @@ __device__ __forceinline__ float sum_groups(float x) {
   return sum_halves(lo + hi);
 }
 
-// The tiles of a sequence are cut into at most `most` pieces of equal length, of at least LEAST tiles (two a wave: below that a
+// The tiles of a sequence are cut into at most `most` pieces of equal length, of at least LEAST tiles (four a wave: below that a
 // workgroup is all start and join).  Short sequences of a ragged batch have few pieces, and the workgroups of the others leave
 // at once; long ones do not get longer pieces than they must.
 constexpr int LEAST = 4 * WAVES;
@@ -236,7 +236,7 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   }
   int mine[NB];                              // where the head's biases start
   float farthest[NB];
-  int lowest = INT_MAX;                      // position of the first query here
+  int lowest = 1 << 30;                      // position of the first query here (none: beyond every row)
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     int hh = qhead[n] - gi0;
@@ -521,7 +521,10 @@ constexpr int BLOCKS = 2;
 Plan plan(const sig3d_decode_attention_args *a) {
   Plan s = {};
   const int group = a->h / a->hkv, per = group * a->t, each = a->groups ? a->b / a->groups : 0;
-  const int reach = a->buckets.n ? device_buckets(a->buckets).reach : 0;
+  const int reach = a->buckets.n ? std::max(1, a->buckets.border[a->buckets.n - 1]) : 0;
+  const int e = a->dtype == 0 ? 4 : 2, row = a->d * e + 32;
+  // V tiles (they also hold the four waves' outputs while these join: 16 rows of d floats each, less), statistics of the join
+  const size_t tiles_bytes = WAVES * KT * row * (a->d == 64 && e == 2 ? 2 : 1) + 2 * WAVES * 16 * 4;
   s.own_tiles = sig3d_ceil_div(per, 16);
   const long base = (long)a->b * a->hkv * s.own_tiles;
   // Walking the shared rows once a sequence costs nothing where no other sequence shares them, and one launch instead of two
@@ -535,7 +538,9 @@ Plan plan(const sig3d_decode_attention_args *a) {
   s.own_splits = (int)std::min<long>(std::max<long>(1, 1024 / base), sig3d_ceil_div(own_rows, LEAST * KT));
   if (each > 0 && !s.joined) {
     const long rows = (long)each * per;
-    s.nb = rows > 16 ? BLOCKS : 1;
+    // (one block of rows where the biases of two would not fit: many heads and a far reach)
+    const size_t biases = a->buckets.n ? (size_t)std::min(group, (16 * BLOCKS + a->t - 2) / a->t + 1) * (reach + 1) * 4 : 0;
+    s.nb = rows > 16 && tiles_bytes + biases <= MOST_LDS ? BLOCKS : 1;
     s.shared_tiles = sig3d_ceil_div(rows, 16 * s.nb);
     const long far = (long)a->groups * a->hkv * s.shared_tiles;
     s.shared_splits = (int)std::min<long>(std::max<long>(1, 256 / far), sig3d_ceil_div(a->shared_capacity, LEAST * KT));
@@ -543,7 +548,6 @@ Plan plan(const sig3d_decode_attention_args *a) {
   }
   s.own_items = (int)(base * s.own_splits);
   s.direct = s.own_splits == 1 && !s.shared_splits;
-  const int e = a->dtype == 0 ? 4 : 2, row = a->d * e + 32;
   if (a->buckets.n) {
     s.own_heads = std::min(group, (16 + a->t - 2) / a->t + 1);
     s.shared_heads = s.shared_splits ? std::min(group, (16 * s.nb + a->t - 2) / a->t + 1) : 0;
@@ -551,9 +555,7 @@ Plan plan(const sig3d_decode_attention_args *a) {
   // One wave an item where a sequence is short: four would start and join for a tile or two each.
   const size_t one = (size_t)WAVES * s.own_heads * (reach + 1) * 4;
   s.wv = one <= 32 * 1024 && (own_rows <= 2 * KT || (base >= 1024 && own_rows <= 16 * KT)) ? 1 : WAVES;
-  // (the V tiles also hold the four waves' outputs while they join: 16 rows of d floats each, less)
-  s.lds = WAVES * KT * row * (a->d == 64 && e == 2 ? 2 : 1) + std::max(s.wv == 1 ? one : s.own_heads * (reach + 1) * 4ul, s.shared_heads * (reach + 1) * 4ul) +
-          2 * WAVES * 16 * 4;
+  s.lds = tiles_bytes + std::max(s.wv == 1 ? one : s.own_heads * (reach + 1) * 4ul, s.shared_heads * (reach + 1) * 4ul);
   return s;
 }
 
@@ -591,7 +593,7 @@ extern "C" int sig3d_decode_attention(const sig3d_decode_attention_args *a, void
   SIG3D_REQUIRE(a->q_b >= 0 && a->q_n >= 0 && a->q_h >= 0 && a->q_b * e % 16 == 0 && a->q_n * e % 16 == 0 && a->q_h * e % 16 == 0,
                 "strides must be non-negative multiples of 16 bytes");
   SIG3D_REQUIRE((long)a->b * a->hkv * s.own_tiles * s.own_splits + s.shared_items < INT_MAX, "grid too large");
-  SIG3D_REQUIRE(s.lds <= 152 * 1024, "bias table too large for LDS");
+  SIG3D_REQUIRE(s.lds <= MOST_LDS, "biases too large for LDS");      // (no call: 16 heads, the longest rows and the farthest reach take 136 KB)
   DecodeParams p = {};
   p.q = a->q; p.table = a->table;
   p.own = {a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->capacity};

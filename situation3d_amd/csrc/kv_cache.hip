@@ -37,22 +37,25 @@ template <typename T, int D> struct Piece {
     if constexpr (LANES == 32) top = fmaxf(top, __shfl_xor(top, 16));
     return top;
   }
-  // A row's e4m3 values, and its scale by its first lane.  Infinities and NaN do not count in the scale; infinities, which only
-  // a wave that has one looks for, become the largest value.
+  // The largest value of 4 significant bits that T holds.  Beyond it the nearest such value may be 2^16 (f16) or 2^128, which
+  // would come back as an infinity: values up to T's largest are brought down to it, by less than 2^-4 of theirs.
+  static constexpr float LIMIT = std::is_same<T, _Float16>::value ? 61440.f : 0x1.ep127f;
+  // A row's e4m3 values, and its scale by its first lane.  Infinities and NaN do not count in the scale; infinities become the
+  // largest value that the scale and T allow.  Only a wave with values beyond LIMIT looks.
   static __device__ __forceinline__ void quantize(unsigned char *to, float *scale, piece x, bool mine, bool first) {
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) top = fmaxf(top, fabsf((float)x[e]));        // fmaxf drops NaN
     top = over_lanes(top);
-    const bool infinite = __any(top == INFINITY);
-    if (infinite) {
+    const bool beyond = __any(top > LIMIT);
+    if (beyond) {
       top = 0.f;
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
         const float a = fabsf((float)x[e]);
         top = a < INFINITY ? fmaxf(top, a) : top;
       }
-      top = over_lanes(top);
+      top = fminf(over_lanes(top), LIMIT);
     }
     // top = m 2^x with m in [0.5, 1), 448 = 0.875 2^9; scales stay normal numbers
     const int ex = __builtin_amdgcn_frexp_expf(top) - 9 + (__builtin_amdgcn_frexp_mantf(top) > 0.875f ? 1 : 0);
@@ -61,9 +64,10 @@ template <typename T, int D> struct Piece {
     float y[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) y[e] = (float)x[e] * inv;
-    if (infinite) {
+    if (beyond) {
+      const float most = fminf(448.f, LIMIT * inv);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) y[e] = fabsf(y[e]) > 448.f ? copysignf(448.f, y[e]) : y[e];
+      for (int e = 0; e < PER; ++e) y[e] = fabsf(y[e]) > most ? copysignf(most, y[e]) : y[e];
     }
     unsigned w[PER / 4];
 #pragma unroll
@@ -144,7 +148,8 @@ template <typename T, int D, bool Q>
 __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
   typedef Piece<T, D> P;
   typedef typename P::piece piece;
-  const int c = blockIdx.x * 256 + threadIdx.x, i = c / P::USED, o = c - i * P::USED;
+  const unsigned c = blockIdx.x * 256 + threadIdx.x;              // below 2^31 + 256: the host looks
+  const int i = c / P::USED, o = c - i * P::USED;
   if (i >= p.n) return;
   const int b = blockIdx.z, head = blockIdx.y;
   piece k{}, v{};
@@ -188,6 +193,8 @@ extern "C" int sig3d_cache_append(const sig3d_cache_append_args *a, void *stream
   SIG3D_REQUIRE((a->k_scale == nullptr) == (a->v_scale == nullptr), "k_scale and v_scale come together");
   SIG3D_REQUIRE(aligned16(a->k) && aligned16(a->v) && aligned16(a->k_cache) && aligned16(a->v_cache),
                 "addresses must be 16-byte aligned");
+  const auto apart = [&](const int *x) { return !x || x + a->b <= a->lengths || x >= a->lengths + a->b; };
+  SIG3D_REQUIRE(apart(a->start) && apart(a->counts), "start and counts must not lie in lengths, which the call writes");
   const int e = a->dtype == 0 ? 4 : 2;
   const long strides[6] = {a->k_b, a->k_n, a->k_h, a->v_b, a->v_n, a->v_h};
   for (long s : strides) SIG3D_REQUIRE(s >= 0 && s * e % 16 == 0, "strides must be non-negative multiples of 16 bytes");

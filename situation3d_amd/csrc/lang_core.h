@@ -223,6 +223,8 @@ template <typename T> struct BiasFill {
     }                                             \
   } while (0)
 
+constexpr size_t MOST_LDS = 152 * 1024;       // of a workgroup, beside its static arrays
+
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 inline int check_buckets(const char *where, const sig3d_rel_buckets &k, const void *table, int table_rows) {
@@ -254,7 +256,7 @@ inline Buckets device_buckets(const sig3d_rel_buckets &k) {
 template <typename K> int allow_lds(K kernel, sig3d_once_per_device &once) {
   if (once.pending()) {
     SIG3D_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      152 * 1024));
+                                      (int)MOST_LDS));
     once.done();
   }
   return 0;

@@ -311,7 +311,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? (D == 128 ? 1 : 2) : D ==
   }
   if (!valid) return;
   l = sum_halves(l);
-  const bool empty = lo >= hi;
+  const bool empty = lo >= hi || (m == -INFINITY && l == 0.f);              // nothing seen, or every bias -inf
   const float inv = empty ? 0.f : 1.f / l;
   const long row = (((long)b * p.nq + qi) * p.h + head) * D;
   if (p.piece) {
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void rel_join_kernel(const Params p) {
 // the diagonal goes through wave-private LDS, one row of 36 floats a distance, element (query i, key j) at [j - i + 31][i]: the
 // addresses are a lane's base plus constants, and lane l then adds row l and puts the sum to its distance -- 64 distances, 64
 // lanes, no two meet and the order of the sums is fixed.  (Adding every element to its distance by an LDS atomic cost 200
-// address and mask instructions and twice the LDS time: 88 us instead of DQ_US for 4 x 32 heads of 432 tokens.)
+// address and mask instructions and twice the LDS time: 88 us instead of 32 for 4 x 32 heads of 432 tokens.)
 constexpr int DIAG_ROW = 36, DIAG = 64 * DIAG_ROW;        // floats; 36: 16-byte rows whose columns spread over the banks
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_kernel(const Params p) {
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D < 128 ? 2 : 1) void re
   const bool biased = p.bk.n > 0;
   const float scale2 = p.scale * LOG2E;
   const int nblocks = (p.nq + 31) / 32, ntiles = (p.nq + QT - 1) / QT;
-  const int4 *blocks = p.blocks + (long)b * ((p.nq + 32 * 4 - 1) / (32 * 4)) * 4;
+  const int4 *blocks = p.blocks + (long)b * p.qtiles * NW;
 
   int up = 0;                                  // f16: dS is held times 2^up, P times 2^P_UP
   if constexpr (narrow<T>()) {

@@ -15,7 +15,6 @@ hkv).  Statistics, sums and gradients' accumulators are float32; results are rou
 stream of their tensors' device, allocate their outputs and workspaces from torch, never synchronise, and may be captured into
 a hipGraph.  GPU tensors only, like the rest of the HIP path.
 """
-import ctypes
 import functools
 import math
 
@@ -108,6 +107,18 @@ def _check_table(shape, dtype, heads, q_dtype, what):
         raise RuntimeError("%s: the bias table is (buckets, heads) = (., %d) in q's type" % (what, heads))
 
 
+def _no_gradient(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("%s has no gradient: call it under torch.no_grad()" % what)
+
+
+def _apart(t, written):
+    """`t`, or a copy of it where it begins in the storage of `written`, which the call to come writes."""
+    if t is None or not 0 <= t.data_ptr() - written.data_ptr() < written.numel() * written.element_size():
+        return t
+    return t.clone()
+
+
 def _int_array(t, shape, device, name):
     if t is None:
         return None
@@ -195,22 +206,23 @@ def _rel_forward(a, q, k, keep, need):
         a.work = work.data_ptr()
     if keep:
         a.out32, a.lse = out32.data_ptr(), lse.data_ptr()
-    _launch("sig3d_rel_attention_fwd", ctypes.byref(a), dev)
+    _launch("sig3d_rel_attention_fwd", a, dev)
     return out, out32, lse
 
 
 class _RelativeAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, cfg, arrays, a, need):
-        out, out32, lse = _rel_forward(a, q, k, True, need)
+    def forward(ctx, q, k, v, table, cfg, arrays, a, work):
+        out, out32, lse = _rel_forward(a, q, k, True, work[0])
         ctx.save_for_backward(q, k, v, table, out32, lse, *arrays)
-        ctx.cfg = cfg
+        ctx.call = cfg, a, work, (q.stride(), k.stride(), v.stride())
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q, k, v, table, out32, lse, *arrays = ctx.saved_tensors
+        cfg, a, work, strides = ctx.call
         dev, dtype = q.device, q.dtype
         dq = torch.empty(q.shape, dtype=dtype, device=dev)
         dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
@@ -220,20 +232,26 @@ class _RelativeAttentionFn(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
             return dq, dk, dv, dtable, None, None, None, None
-        a, ok, work = _rel_args(q, k, v, table, ctx.cfg, arrays)
-        if not ok:                               # saved tensors came back laid out differently (hooks)
-            q, k, v = _rows(q), _rows(k), _rows(v)
-            a, _, work = _rel_args(q, k, v, table, ctx.cfg, arrays)
+        if (q.data_ptr(), k.data_ptr(), v.data_ptr()) == (a.q, a.k, a.v) and (q.stride(), k.stride(), v.stride()) == strides:
+            a = _lib.RelAttentionArgs.from_buffer_copy(a)
+        else:                                    # saved tensors came back from elsewhere (hooks)
+            a, ok, work = _rel_args(q, k, v, table, cfg, arrays)
+            if not ok:
+                q, k, v = _rows(q), _rows(k), _rows(v)
+                a, _, work = _rel_args(q, k, v, table, cfg, arrays)
         grad = _rows(grad)
         a.grad_b, a.grad_n, a.grad_h = _strides(grad.shape, grad.stride())
         # (out is not read again: the kernels take the unrounded copy; its address only has to be one)
-        a.out, a.out32, a.lse, a.grad = out32.data_ptr(), out32.data_ptr(), lse.data_ptr(), grad.data_ptr()
-        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        a.out = a.out32 = out32.data_ptr()
+        a.lse, a.grad, a.dq, a.dk, a.dv = lse.data_ptr(), grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if dtable is not None:
-            a.dtable = dtable.data_ptr()
+            a.table, a.dtable = table.data_ptr(), dtable.data_ptr()
+        for name, x in zip(("key_lengths", "prefix_lengths", "key_ranges"), arrays):
+            if x is not None:
+                setattr(a, name, x.data_ptr())
         work = torch.empty(work[1], dtype=torch.float32, device=dev)
         a.work = work.data_ptr()
-        _launch("sig3d_rel_attention_bwd", ctypes.byref(a), dev)
+        _launch("sig3d_rel_attention_bwd", a, dev)
         return dq, dk, dv, dtable, None, None, None, None
 
 
@@ -248,10 +266,16 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
       bucket 0.  T5 does not scale: pass scale=1.0 there; None is d ** -0.5.
     What a query sees: j < key_lengths[b] (b,), and with causal j <= p or j < prefix_lengths[b] (b,), and
       key_ranges[b, i, 0] <= j < key_ranges[b, i, 1] (b, nq, 2), all int32 on q's device; None does not restrict.  A query that
-      sees nothing yields 0 and passes no gradient.  Keys that no query sees may hold anything; a key that some query sees
-      must be finite for the others.
+      sees nothing yields 0 and passes no gradient.  Keys before the first and behind the last that any query of the sequence
+      sees may hold anything; those between are finite, also for queries that do not see them.
+    A bias of -inf weighs nothing, and neither do float32's and bfloat16's lowest values; a query that sees only such keys
+      yields 0 as well.
     -> (b, nq, h, d) in q's type."""
-    dev = _lib.require_device(q, k, v, table, key_lengths, prefix_lengths, key_ranges)
+    dev = q.device
+    if not q.is_cuda:
+        raise RuntimeError("CPU not supported")
+    if k.device != dev or v.device != dev or table is not None and table.device != dev:
+        raise RuntimeError("all tensors must be on the same device")
     if prefix_lengths is not None and not causal:
         raise RuntimeError("relative_attention: prefix_lengths only means something with causal=True")
     cfg = (float(q.shape[-1] ** -0.5 if scale is None else scale), bool(bidirectional), int(max_distance), bool(causal),
@@ -273,7 +297,7 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
         a, _, work = _rel_args(q, k, v, table, cfg, arrays)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or table is not None and table.requires_grad):
-        return _RelativeAttentionFn.apply(q, k, v, table, cfg, arrays, a, work[0])
+        return _RelativeAttentionFn.apply(q, k, v, table, cfg, arrays, a, work)
     return _rel_forward(a, q, k, False, work[0])[0]
 
 
@@ -284,7 +308,7 @@ class KVCache:
     max |x| <= 448 scale -- half the bytes of bfloat16; one rounding to 4 significant bits, at most 2^-4 of a value.  Else held
     in `dtype`.  Attributes: k, v (batch, capacity, kv_heads, head_dim), k_scale, v_scale (batch, capacity, kv_heads) or
     None, lengths (batch,) int32 -- tensors of fixed address that the program may read and write (scales must stay powers of
-    two), and that captured graphs may keep using.  They are views of head-major storage."""
+    two), and that captured graphs may keep using.  They are views of head-major storage.  Inference only: no gradients."""
 
     def __init__(self, batch, capacity, kv_heads, head_dim, dtype=torch.bfloat16, quantized=False, device="cuda"):
         device = torch.device(device)
@@ -301,17 +325,22 @@ class KVCache:
         self._ks = self._vs = None
         if quantized:
             self._ks, self._vs = (torch.ones((batch, kv_heads, capacity), dtype=torch.float32, device=device) for _ in range(2))
-        self.k, self.v = self._k.transpose(1, 2), self._v.transpose(1, 2)
-        self.k_scale = self._ks.transpose(1, 2) if quantized else None
-        self.v_scale = self._vs.transpose(1, 2) if quantized else None
-        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
-        self.device = self.lengths.device
+        self._lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.device = self._lengths.device
+
+    # (nothing to assign to: the kernels use the storage)
+    k = property(lambda self: self._k.transpose(1, 2))
+    v = property(lambda self: self._v.transpose(1, 2))
+    k_scale = property(lambda self: None if self._ks is None else self._ks.transpose(1, 2))
+    v_scale = property(lambda self: None if self._vs is None else self._vs.transpose(1, 2))
+    lengths = property(lambda self: self._lengths)
 
     def append(self, k, v, start=None, counts=None):
         """Tokens k, v (batch, t, kv_heads, head_dim) in the cache's type: the first counts[b] (None: t) go to rows
         start[b] + i (None: behind what is there), and lengths[b] becomes start[b] + counts[b]; both int32 (batch,).  Tokens
         beyond the capacity are dropped and lengths stops there; other rows stay as they are."""
-        dev = _lib.require_device(self.lengths, k, v, start, counts)
+        dev = _lib.require_device(self._lengths, k, v, start, counts)
+        _no_gradient("KVCache.append", k, v)
         if k.dim() != 4 or k.shape != v.shape or k.shape[0] != self.batch or k.shape[2] != self.kv_heads or k.shape[3] != self.head_dim:
             raise RuntimeError("KVCache.append: k and v must be (%d, t, %d, %d)" % (self.batch, self.kv_heads, self.head_dim))
         if k.dtype != self.dtype or v.dtype != self.dtype:
@@ -320,14 +349,16 @@ class KVCache:
         t = k.shape[1]
         if t == 0:
             if start is not None:
-                self.lengths.copy_(start.clamp(0, self.capacity))
+                self._lengths.copy_(start.clamp(0, self.capacity))
             return
-        k, v = _rows(k), _rows(v)
+        # what the call writes is not read beside it
+        start, counts = _apart(start, self._lengths), _apart(counts, self._lengths)
+        k, v = _rows(_apart(_apart(k, self._k), self._v)), _rows(_apart(_apart(v, self._k), self._v))
         a = _lib.CacheAppendArgs(k.data_ptr(), v.data_ptr(), self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs),
-                                 _ptr(start), _ptr(counts), self.lengths.data_ptr(), *_strides(k.shape, k.stride()),
+                                 _ptr(start), _ptr(counts), self._lengths.data_ptr(), *_strides(k.shape, k.stride()),
                                  *_strides(v.shape, v.stride()), _DTYPES[self.dtype], self.batch, t, self.capacity, self.kv_heads,
                                  self.head_dim)
-        _launch("sig3d_cache_append", ctypes.byref(a), dev)
+        _launch("sig3d_cache_append", a, dev)
 
     def read(self, tokens=None):
         """(k, v) (batch, tokens, kv_heads, head_dim) in the cache's type: the values that the first `tokens` rows (None: all)
@@ -338,10 +369,10 @@ class KVCache:
         shape = (self.batch, n, self.kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device)
         if n:
-            a = _lib.CacheReadArgs(self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs), self.lengths.data_ptr(),
+            a = _lib.CacheReadArgs(self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs), self._lengths.data_ptr(),
                                    k.data_ptr(), v.data_ptr(), _DTYPES[self.dtype], self.batch, n, self.capacity, self.kv_heads,
                                    self.head_dim)
-            _launch("sig3d_cache_read", ctypes.byref(a), self.device)
+            _launch("sig3d_cache_read", a, self.device)
         return k, v
 
 
@@ -354,9 +385,11 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
       and before its own tokens -- b / g questions about one scene, read from memory once for all of them.
     table as in relative_attention (keys are never ahead of the query, so bidirectional only says which half of the table
       counts); positions count the shared tokens first.
+    Rows of a cache from its length on may hold anything.
     -> (b, t, h, d) in q's type."""
-    dev = _lib.require_device(q, cache.lengths, None if shared is None else shared.lengths, table, counts)
+    dev = _lib.require_device(q, cache._lengths, None if shared is None else shared._lengths, table, counts)
     what = "decode_attention"
+    _no_gradient(what, q, table)
     if q.dim() != 4 or q.dtype != cache.dtype:
         raise RuntimeError("%s: q is (batch, new tokens, heads, head size) in the cache's type" % what)
     b, t, h, d = shape = q.shape
@@ -381,11 +414,11 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
                                float(d ** -0.5 if scale is None else scale), int(max_distance), bool(bidirectional))
     a = _lib.DecodeAttentionArgs.from_buffer_copy(a)
     a.q, a.out, a.k_cache, a.v_cache = q.data_ptr(), out.data_ptr(), cache._k.data_ptr(), cache._v.data_ptr()
-    a.lengths = cache.lengths.data_ptr()
+    a.lengths = cache._lengths.data_ptr()
     if cache.quantized:
         a.k_scale, a.v_scale = cache._ks.data_ptr(), cache._vs.data_ptr()
     if shared is not None:
-        a.shared_k, a.shared_v, a.shared_lengths = shared._k.data_ptr(), shared._v.data_ptr(), shared.lengths.data_ptr()
+        a.shared_k, a.shared_v, a.shared_lengths = shared._k.data_ptr(), shared._v.data_ptr(), shared._lengths.data_ptr()
         if cache.quantized:
             a.shared_k_scale, a.shared_v_scale = shared._ks.data_ptr(), shared._vs.data_ptr()
     if rows:
@@ -395,7 +428,7 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
     if need:
         work = torch.empty(need, dtype=torch.float32, device=dev)
         a.work = work.data_ptr()
-    _launch("sig3d_decode_attention", ctypes.byref(a), dev)
+    _launch("sig3d_decode_attention", a, dev)
     return out
 
 

@@ -137,7 +137,7 @@ def test_null_arguments_are_refused():
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=5), dict(b=0), dict(b=70000), dict(t=0), dict(capacity=0), dict(hkv=0), dict(d=72), dict(k=0),
-                                 dict(v_cache=0), dict(lengths=0), dict(k_scale=0), dict(k=A + 1), dict(k_n=7), dict(v_h=-8),
+                                 dict(v_cache=0), dict(lengths=0), dict(start=A), dict(counts=A), dict(k_scale=0), dict(k=A + 1), dict(k_n=7), dict(v_h=-8),
                                  dict(t=1 << 29, hkv=2)], ids=str)
 def test_cache_append_refuses(bad):
     from situation3d_amd import _lib

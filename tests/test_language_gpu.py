@@ -49,6 +49,8 @@ ATTENTION = [
     (1, 70, 70, 2, 2, 64, dict(buckets=2, max_distance=5, bidirectional=False)),
     (1, 600, 640, 1, 1, 64, dict(buckets=64, max_distance=1000, scale=1.0)),
     (2, 100, 100, 2, 2, 64, dict(key_ranges=True)),
+    (2, 150, 2100, 4, 2, 96, dict(key_lengths=(2100, 300), causal=True, query_offset=1950, bidirectional=False)),     # runs of keys
+    (2, 1100, 200, 8, 2, 128, dict(key_lengths=(200, 130))),                                       # runs of queries, heads apart
 ]
 
 
@@ -321,6 +323,41 @@ def test_reading_and_writing_back_changes_nothing():
     assert all(torch.equal(x, y) for x, y in zip(a.read(), b.read()))
 
 
+def test_append_reads_what_it_moves():
+    """`start` and `counts` may be the lengths that the call moves, k and v rows of the cache itself."""
+    lang = _lang()
+    g = torch.Generator().manual_seed(8)
+    cache = lang.KVCache(2, 700, 4, 64, torch.bfloat16, False, DEV)
+    x, y = (_randn(g, 2, 300, 4, 64, dtype=torch.bfloat16) for _ in range(2))
+    cache.append(x, y, counts=_i32(300, 40))
+    cache.append(x, y, start=cache.lengths, counts=cache.lengths)          # as many once more
+    assert cache.lengths.tolist() == [600, 80]
+    for i, n in enumerate((300, 40)):
+        assert torch.equal(cache.k[i, :2 * n], torch.cat([x[i, :n]] * 2)) and torch.equal(cache.v[i, :2 * n], torch.cat([y[i, :n]] * 2))
+    before = cache.k.clone(), cache.v.clone()
+    cache.append(cache.k[:, :500], cache.v[:, :500], start=_i32(1, 1))     # every row one further
+    assert cache.lengths.tolist() == [501, 501]
+    for now, was in zip((cache.k, cache.v), before):                       # as bits: some rows were never written
+        assert torch.equal(now[:, 1:501].view(torch.int16), was[:, :500].view(torch.int16))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_cache_values_near_the_largest(dtype):
+    """What a type holds comes back finite and within 2^-4 of itself; an infinity as the largest value there is."""
+    top = torch.finfo(dtype).max
+    cache = _lang().KVCache(1, 3, 1, 96, dtype, True, DEV)
+    k = torch.zeros(1, 3, 1, 96, dtype=dtype)
+    k[0, 0, 0, :5] = torch.tensor([top, -top, top * 0.97, top * 0.9, top / 3], dtype=dtype)
+    k[0, 1, 0, :3] = torch.tensor([math.inf, -math.inf, top], dtype=dtype)
+    k[0, 2, 0, 17] = top * 0.94
+    cache.append(k.to(DEV), k.to(DEV))
+    for got in cache.read():
+        got, want = got[0, :, 0].cpu().double(), k[0, :, 0].double()
+        assert got.isfinite().all()
+        assert ((got - want).abs() <= 2.0 ** -4 * want.abs())[[0, 2]].all() and not got[1, 3:].any()
+        assert got[1, 0] == got[1, 2] == -got[1, 1] and abs(got[1, 2] / top - 1) <= 2.0 ** -4
+
+
 # ---- decoding ------------------------------------------------------------------------------------------------------------
 
 def _filled(g, n, capacity, hkv, d, dtype, quantized, lengths, rubbish=True):
@@ -473,6 +510,87 @@ def test_a_captured_decoding_step_replays():
         assert caches[0].lengths.tolist() == [i + 1] * b == caches[1].lengths.tolist()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_many_heads_with_a_far_reach_over_shared_rows(dtype):
+    """The biases of 32 query rows of as many heads would not fit into LDS."""
+    _check_decode(torch.Generator().manual_seed(9), b=2, t=1, h=32, hkv=1, d=128, capacity=40, lengths=(33, 4), dtype=dtype,
+                  quantized=False, groups=1, prefix=(560,), shared_capacity=600, buckets=64, max_distance=1024)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_biases_of_minus_infinity_weigh_nothing(dtype):
+    """-inf (or a lowest value that becomes one): the key is as if masked, and a query with nothing else yields 0."""
+    lowest = -math.inf if dtype == torch.float16 else torch.finfo(dtype).min
+    for b, nq, nk, offset, buckets in ((2, 200, 200, 0, (0,)), (1, 70, 2000, 1930, (5, 31)), (1, 40, 40, 0, tuple(range(32)))):
+        case = (b, nq, nk, 4, 2, 64, dict(causal=True, query_offset=offset, bidirectional=False))
+        q, k, v, table, grad, ok, index, opts = _attention_case(case, dtype, nq)
+        table[list(buckets)] = 0
+        for bucket in buckets:
+            ok = ok & (index != bucket)
+        want = ref.attention(q, k, v, table, ok, 0.125, index, grad)
+        for value in (-math.inf, lowest):
+            table[list(buckets)] = value
+            leaves = [x.detach().requires_grad_() for x in (q, k, v, table)]
+            out = _lang().relative_attention(*leaves, **opts)
+            ref.check("out", out, want["out"])
+            for name, x in zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(out, leaves, grad)):
+                ref.check(name, x, want[name])
+
+
+def test_saved_tensors_may_move():
+    g = torch.Generator().manual_seed(10)
+    q, k, v = (_randn(g, 2, 90, 4, 64, dtype=torch.bfloat16).requires_grad_() for _ in range(3))
+    table, grad = _randn(g, 32, 4, dtype=torch.bfloat16).requires_grad_(), _randn(g, 2, 90, 4, 64, dtype=torch.bfloat16)
+    call = lambda: _lang().relative_attention(q, k, v, table, causal=True, key_lengths=_i32(90, 31))          # noqa: E731
+    want = torch.autograd.grad(call(), [q, k, v, table], grad)
+    with torch.autograd.graph.save_on_cpu():
+        out = call()
+    filler = [torch.full((2, 90, 4, 64), math.nan, device=DEV) for _ in range(8)]      # where the saved ones were
+    got = torch.autograd.grad(out, [q, k, v, table], grad)
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and filler
+    out = call()
+    for _ in range(2):                                                                  # and are read as often as asked
+        got = torch.autograd.grad(out, [q, k, v, table], grad, retain_graph=True)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_addresses_beyond_32_bits():
+    """Token strides of 8 MB: the last rows of 600 lie 5 GB behind the first."""
+    n, stride = 600, 1 << 22
+    x = torch.zeros(n * stride + 1024, dtype=torch.bfloat16, device=DEV)
+    q, k, v = (x.as_strided((1, n, 2, 64), (n * stride, stride, 64, 1), 128 * i) for i in range(3))
+    g = torch.Generator().manual_seed(11)
+    dense = [_randn(g, 1, n, 2, 64, dtype=torch.bfloat16) for _ in range(3)]
+    for to, of in zip((q, k, v), dense):
+        to.copy_(of)
+    grad = _randn(g, 1, n, 2, 64, dtype=torch.bfloat16)
+    leaves = [[t.detach().requires_grad_() for t in ts] for ts in ((q, k, v), dense)]
+    outs = [_lang().relative_attention(*ts, causal=True) for ts in leaves]
+    assert torch.equal(*outs)
+    for a, b in zip(*(torch.autograd.grad(out, ts, grad) for out, ts in zip(outs, leaves))):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("quantized", [False, True], ids=["plain", "e4m3"])
+def test_long_caches(quantized):
+    """Heads of 4 GB: one key of the last head's last rows has all the weight (60 against 0: the others' is e^-60 2^25)."""
+    capacity = 1 << (25 if quantized else 24)
+    cache = _lang().KVCache(1, capacity, 3, 128, torch.bfloat16, quantized, DEV)
+    cache._k.view(torch.uint8).zero_()
+    cache._v.view(torch.uint8).zero_()
+    k, v = torch.zeros(1, 2, 3, 128, device=DEV, dtype=torch.bfloat16), torch.zeros(1, 2, 3, 128, device=DEV, dtype=torch.bfloat16)
+    k[0, 0, :, 0] = 64
+    v[0, 0] = torch.arange(3 * 128, device=DEV).reshape(3, 128) % 13 + 1
+    cache.append(k, v, start=_i32(capacity - 2))
+    q = torch.zeros(1, 1, 6, 128, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 1
+    got = _lang().decode_attention(q, cache, scale=60 / 64)
+    assert torch.equal(got[0, 0], v[0, 0].repeat_interleave(2, 0))
+    cache.append(k, v, start=_i32(0))
+    assert torch.equal(_lang().decode_attention(q, cache, scale=60 / 64)[0, 0], v[0, 0].repeat_interleave(2, 0))
+    assert torch.equal(cache.k[0, -2:].float(), k[0].float() / (cache.k_scale[0, -2:, :, None] if quantized else 1))
+
+
 def test_gpu_refusals():
     lang = _lang()
     x = torch.zeros(2, 4, 4, 64, device=DEV, dtype=torch.bfloat16)
@@ -492,6 +610,9 @@ def test_gpu_refusals():
                 lambda: lang.decode_attention(x.float(), cache), lambda: lang.decode_attention(x[:1], cache),
                 lambda: lang.decode_attention(x, cache, lang.KVCache(2, 8, 4, 64, torch.bfloat16, True, DEV)),
                 lambda: lang.decode_attention(x, cache, lang.KVCache(3, 8, 4, 64, torch.bfloat16, False, DEV)),
-                lambda: lang.decode_attention(x, cache, None, torch.zeros(32, 4, device=DEV))):
+                lambda: lang.decode_attention(x, cache, None, torch.zeros(32, 4, device=DEV)),
+                lambda: lang.decode_attention(x.clone().requires_grad_(), cache), lambda: cache.append(x, x.clone().requires_grad_())):
         with pytest.raises(RuntimeError):
             bad()
+    with pytest.raises(AttributeError):
+        cache.lengths = _i32(1, 1)
