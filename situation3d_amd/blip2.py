@@ -9,7 +9,7 @@ queries, cross-attention to the point tokens) -> `t5_proj`.
 
 The frozen Flan-T5-XL that turns `inputs_t5` into the loss (blip2_t5.py:136-183) is out of scope
 (3 B parameters, weights unavailable); plug it in as `language_head(inputs_t5, atts_t5, samples)
--> loss`.  Without one, "loss" is None.
+-> loss` (language.py has the operators to build one from).  Without one, "loss" is None.
 
 The reference builds the position term on the CPU in a Python double loop and copies
 B x N x 1408 floats to the GPU every step (blip2_t5.py:106-116); here it is one streaming HIP

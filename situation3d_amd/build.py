@@ -45,7 +45,7 @@ def build(force=False, verbose=False):
     hipcc = _hipcc()
     jobs = []
     # longest compile first (measured, seconds on one core of the build container; the rest by size)
-    cost = {"shared_mlp_fwd4r.hip": 44, "gemmp.hip": 33, "shared_mlp_fwd2.hip": 30, "gemm16.hip": 26,
+    cost = {"decode_attention.hip": 55, "shared_mlp_fwd4r.hip": 44, "rel_attention.hip": 29, "gemmp.hip": 33, "shared_mlp_fwd2.hip": 30, "gemm16.hip": 26,
             "shared_mlp_fwd4.hip": 21, "shared_mlp_fwd1.hip": 18, "shared_mlp.hip": 13}
     for src in sorted(SOURCES, key=lambda f: -cost.get(f, os.path.getsize(os.path.join(CSRC, f)) / 2e4)):
         s = os.path.join(CSRC, src)
@@ -59,7 +59,7 @@ def build(force=False, verbose=False):
         subprocess.check_call(cmd)
 
     if jobs:
-        # the longest translation unit (shared_mlp_fwd4r.hip, ~45 s alone) bounds the wall time once every file has a core
+        # the longest translation unit (decode_attention.hip, ~55 s alone) bounds the wall time once every file has a core
         with ThreadPoolExecutor(max_workers=min(os.cpu_count() or 4, 8, len(jobs))) as ex:
             list(ex.map(run, jobs))
     objs = [os.path.join(OBJ, s.replace(".hip", ".o")) for s in SOURCES]
