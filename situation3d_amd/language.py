@@ -69,14 +69,19 @@ def _readable(shape, stride, itemsize):
 
 
 def _strides(shape, stride):
-    return [0 if n == 1 else s for n, s in zip(shape[:-1], stride[:-1])]
+    b, n, h, _ = shape
+    return 0 if b == 1 else stride[0], 0 if n == 1 else stride[1], 0 if h == 1 else stride[2]
 
 
 def _rows(t):
     """`t`, or a dense copy where the kernels cannot read its rows (differentiable)."""
-    if t.data_ptr() % 16 == 0 and _readable(t.shape, t.stride(), t.element_size()):
+    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or _readable(t.shape, t.stride(), t.element_size())):
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _new(like, dtype=None):
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _launch(name, args, device):
@@ -112,17 +117,10 @@ def _no_gradient(what, *tensors):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad()" % what)
 
 
-def _apart(t, written):
-    """`t`, or a copy of it where it begins in the storage of `written`, which the call to come writes."""
-    if t is None or not 0 <= t.data_ptr() - written.data_ptr() < written.numel() * written.element_size():
-        return t
-    return t.clone()
-
-
 def _int_array(t, shape, device, name):
     if t is None:
         return None
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device:
+    if t.dtype != torch.int32 or t.shape != shape or t.device != device:
         raise RuntimeError("%s must be an int32 tensor of shape %s on %s" % (name, shape, device))
     return t.contiguous()
 
@@ -190,11 +188,11 @@ def _rel_args(q, k, v, table, cfg, arrays):
 
 
 def _rel_forward(a, q, k, keep, need):
-    b, nq, h, d = shape = q.shape
+    b, nq, h, _ = q.shape
     dev = q.device
-    out = torch.empty(shape, dtype=q.dtype, device=dev)
+    out = _new(q)
     # the unrounded output: delta = dO.O decides dS where one key has almost all of a row, and O rounded to 8 bits would not do
-    out32 = torch.empty(shape, dtype=torch.float32, device=dev) if keep else None
+    out32 = _new(q, torch.float32) if keep else None
     lse = torch.empty((b, h, nq), dtype=torch.float32, device=dev) if keep else None
     if out.numel() == 0:
         return out, out32, lse
@@ -223,10 +221,8 @@ class _RelativeAttentionFn(torch.autograd.Function):
     def backward(ctx, grad):
         q, k, v, table, out32, lse, *arrays = ctx.saved_tensors
         cfg, a, work, strides = ctx.call
-        dev, dtype = q.device, q.dtype
-        dq = torch.empty(q.shape, dtype=dtype, device=dev)
-        dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
-        dtable = None if table is None else torch.empty(table.shape, dtype=dtype, device=dev)
+        dev = q.device
+        dq, dk, dv, dtable = _new(q), _new(k), _new(v), None if table is None else _new(table)
         if q.numel() == 0 or k.numel() == 0:
             for t in (dq, dk, dv, dtable):
                 if t is not None:
@@ -327,6 +323,18 @@ class KVCache:
             self._ks, self._vs = (torch.ones((batch, kv_heads, capacity), dtype=torch.float32, device=device) for _ in range(2))
         self._lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.device = self._lengths.device
+        # where the storage lies (what an append writes is not read beside it), and the calls' arguments without the tokens'
+        self._spans = [(x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in (self._k, self._v, self._lengths)]
+        self._append = _lib.CacheAppendArgs(
+            k_cache=self._k.data_ptr(), v_cache=self._v.data_ptr(), k_scale=_ptr(self._ks), v_scale=_ptr(self._vs),
+            lengths=self._lengths.data_ptr(), dtype=_DTYPES[dtype], b=batch, capacity=capacity, hkv=kv_heads, d=head_dim)
+        self._read = _lib.CacheReadArgs(
+            k_cache=self._k.data_ptr(), v_cache=self._v.data_ptr(), k_scale=_ptr(self._ks), v_scale=_ptr(self._vs),
+            lengths=self._lengths.data_ptr(), dtype=_DTYPES[dtype], b=batch, capacity=capacity, hkv=kv_heads, d=head_dim)
+
+    def _apart(self, t):
+        p = t.data_ptr()
+        return t.clone() if any(lo <= p < hi for lo, hi in self._spans) else t
 
     # (nothing to assign to: the kernels use the storage)
     k = property(lambda self: self._k.transpose(1, 2))
@@ -339,25 +347,34 @@ class KVCache:
         """Tokens k, v (batch, t, kv_heads, head_dim) in the cache's type: the first counts[b] (None: t) go to rows
         start[b] + i (None: behind what is there), and lengths[b] becomes start[b] + counts[b]; both int32 (batch,).  Tokens
         beyond the capacity are dropped and lengths stops there; other rows stay as they are."""
-        dev = _lib.require_device(self._lengths, k, v, start, counts)
-        _no_gradient("KVCache.append", k, v)
-        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != self.batch or k.shape[2] != self.kv_heads or k.shape[3] != self.head_dim:
+        dev = self.device
+        if not k.is_cuda or not v.is_cuda:
+            raise RuntimeError("CPU not supported")
+        if k.device != dev or v.device != dev:
+            raise RuntimeError("all tensors must be on the same device")
+        if k.requires_grad or v.requires_grad:
+            _no_gradient("KVCache.append", k, v)
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or shape[0] != self.batch or shape[2:] != (self.kv_heads, self.head_dim):
             raise RuntimeError("KVCache.append: k and v must be (%d, t, %d, %d)" % (self.batch, self.kv_heads, self.head_dim))
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise RuntimeError("KVCache.append: the cache takes %s" % self.dtype)
         start, counts = _int_array(start, (self.batch,), dev, "start"), _int_array(counts, (self.batch,), dev, "counts")
-        t = k.shape[1]
-        if t == 0:
+        if shape[1] == 0:
             if start is not None:
                 self._lengths.copy_(start.clamp(0, self.capacity))
             return
-        # what the call writes is not read beside it
-        start, counts = _apart(start, self._lengths), _apart(counts, self._lengths)
-        k, v = _rows(_apart(_apart(k, self._k), self._v)), _rows(_apart(_apart(v, self._k), self._v))
-        a = _lib.CacheAppendArgs(k.data_ptr(), v.data_ptr(), self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs),
-                                 _ptr(start), _ptr(counts), self._lengths.data_ptr(), *_strides(k.shape, k.stride()),
-                                 *_strides(v.shape, v.stride()), _DTYPES[self.dtype], self.batch, t, self.capacity, self.kv_heads,
-                                 self.head_dim)
+        k, v = _rows(self._apart(k)), _rows(self._apart(v))
+        a = _lib.CacheAppendArgs.from_buffer_copy(self._append)
+        a.t, a.k, a.v = shape[1], k.data_ptr(), v.data_ptr()
+        a.k_b, a.k_n, a.k_h = _strides(shape, k.stride())
+        a.v_b, a.v_n, a.v_h = _strides(shape, v.stride())
+        if start is not None:
+            start = self._apart(start)
+            a.start = start.data_ptr()
+        if counts is not None:
+            counts = self._apart(counts)
+            a.counts = counts.data_ptr()
         _launch("sig3d_cache_append", a, dev)
 
     def read(self, tokens=None):
@@ -366,12 +383,11 @@ class KVCache:
         n = self.capacity if tokens is None else int(tokens)
         if not 0 <= n <= self.capacity:
             raise RuntimeError("KVCache.read: %d of %d rows" % (n, self.capacity))
-        shape = (self.batch, n, self.kv_heads, self.head_dim)
-        k, v = torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device)
+        k = torch.empty((self.batch, n, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        v = torch.empty_like(k)
         if n:
-            a = _lib.CacheReadArgs(self._k.data_ptr(), self._v.data_ptr(), _ptr(self._ks), _ptr(self._vs), self._lengths.data_ptr(),
-                                   k.data_ptr(), v.data_ptr(), _DTYPES[self.dtype], self.batch, n, self.capacity, self.kv_heads,
-                                   self.head_dim)
+            a = _lib.CacheReadArgs.from_buffer_copy(self._read)
+            a.k_out, a.v_out, a.n = k.data_ptr(), v.data_ptr(), n
             _launch("sig3d_cache_read", a, self.device)
         return k, v
 
@@ -387,9 +403,13 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
       counts); positions count the shared tokens first.
     Rows of a cache from its length on may hold anything.
     -> (b, t, h, d) in q's type."""
-    dev = _lib.require_device(q, cache._lengths, None if shared is None else shared._lengths, table, counts)
-    what = "decode_attention"
-    _no_gradient(what, q, table)
+    dev, what = cache.device, "decode_attention"
+    if not q.is_cuda or table is not None and not table.is_cuda:
+        raise RuntimeError("CPU not supported")
+    if q.device != dev or shared is not None and shared.device != dev or table is not None and table.device != dev:
+        raise RuntimeError("all tensors must be on the same device")
+    if q.requires_grad or table is not None and table.requires_grad:
+        _no_gradient(what, q, table)
     if q.dim() != 4 or q.dtype != cache.dtype:
         raise RuntimeError("%s: q is (batch, new tokens, heads, head size) in the cache's type" % what)
     b, t, h, d = shape = q.shape
@@ -405,7 +425,7 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
         table, rows = table.contiguous(), table.shape[0]
     if counts is not None:
         counts = _int_array(counts, (b,), dev, "counts")
-    out = torch.empty(shape, dtype=q.dtype, device=dev)
+    out = _new(q)
     if t == 0:
         return out
     q = _rows(q)
