@@ -29,7 +29,9 @@ struct Params {
   const void *q, *k, *v, *table, *grad;
   const int *key_lengths, *prefix_lengths, *key_ranges;
   void *out, *dq, *dk, *dv, *dtable;
-  float *out32, *lse, *delta, *hist;
+  float *out32, *lse, *hist;
+  float2 *stat;                               // backward: lse, delta of a query and head
+  int2 *rows;                                 // backward: first key and number of keys that a query sees
   float *part;                                // backward: dK, dV of every split, (2, splits, b, nk, hkv, d), or NULL: one split
   float *piece, *piece_ml;                    // one output, maximum and sum (forward), one dQ for every key split, or NULL
   int4 *blocks;                               // backward: interval summary of every 32 queries
@@ -144,6 +146,9 @@ template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32
 template <typename T> constexpr int dq_tile(int d) { return sizeof(T) == 2 && d == 64 ? 64 : 32; }
 // queries of a tile of the dK / dV kernel, likewise (at 128 wide K, V and both sums fill a SIMD with one wave anyway)
 template <typename T> constexpr int dkv_tile(int d) { return sizeof(T) == 2 && d != 96 ? 64 : 32; }
+// At 96 wide that kernel's K rows stay in LDS: with V and both sums they are more than two waves' registers (2 x 4096 packed bf16
+// tokens, 16 heads on 4: 160 us instead of 170; at 128 wide they would be 37 registers over even so, and 250 us instead of 197).
+template <typename T> constexpr bool dkv_keys_in_lds(int d) { return sizeof(T) == 2 && d == 96; }
 
 // s (scaled scores of a 32 x 32 block, in log2 units) += bias.  first = position of register 0's row minus that of the lane's
 // column, i.e. register r stands at relative position first + sign * (16 (r >> 3) + (r & 7)).
@@ -441,8 +446,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
     for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[s][j], x[j], delta);
   }
   delta = sum_halves(delta);
+  if (valid && half == 0 && split == 0) {
+    p.stat[stat] = make_float2(lse, delta);
+    if (head == 0) p.rows[(long)b * p.nq + qi] = make_int2(lo, hi - lo);
+  }
   if (!valid) lse = INFINITY;
-  if (valid && half == 0 && split == 0) p.delta[stat] = delta;
   float undo = 1.f;                                       // dS is held times 1 / undo
   if constexpr (narrow<T>()) {
     float top = 0.f;
@@ -611,7 +619,8 @@ __global__ __launch_bounds__(256) void rel_bwd_table_kernel(const float *hist, i
 
 // ---- backward: dK, dV --------------------------------------------------------------------------------------------------------
 // A wave owns 32 keys (columns; K and V rows in registers), a workgroup NW waves that share the streamed query tiles (Q, dO,
-// lse, delta, intervals).  S = Q K^T, dP = dO V^T with queries along the registers: P and dS are at once the B operands of
+// lse, delta, intervals; the last three made ready by the dQ kernel: computed here, behind loads of their own, they had every
+// tile wait for memory -- 245 us instead of 197 for packed documents of 128 wide heads, 35 instead of 31 for the encoder's).  S = Q K^T, dP = dO V^T with queries along the registers: P and dS are at once the B operands of
 // dV^T += dO^T P and dK^T += Q^T dS.  The heads that share the keys are a loop: their sums stay in the accumulators -- unless
 // there are too few workgroups for the chip (see splits_of): then heads and runs of queries become workgroups of their own,
 // which leave f32 sums that a small kernel adds in order.
@@ -623,7 +632,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D < 128 ? 2 : 1) void re
   __shared__ float stats[2][2][QT];            // [buffer][lse, delta]
   __shared__ int rows[2][2][QT];               // [buffer][lo, hi]
   __shared__ int todo[256], ntodo;
-  float *bias = reinterpret_cast<float *>(lds + 4 * TB);
+  constexpr bool KL = dkv_keys_in_lds<T>(D);
+  float *bias = reinterpret_cast<float *>(lds + 4 * TB + (KL ? NW * 32 * TL::ROW : 0));
   const int reach = p.bk.reach;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
@@ -638,6 +648,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D < 128 ? 2 : 1) void re
   const int krow = min(key, p.nk - 1);
   load_row<T, D>(kf, reinterpret_cast<const T *>(p.k) + b * p.k_b + (long)krow * p.k_n + kvh * p.k_h, half);
   load_row<T, D>(vf, reinterpret_cast<const T *>(p.v) + b * p.v_b + (long)krow * p.v_n + kvh * p.v_h, half);
+  char *const ktile = lds + 4 * TB + wave * 32 * TL::ROW;      // this wave's, a lane's row at kappa(col): conflict-free as ever
+  if constexpr (KL) {
+#pragma unroll
+    for (int f = 0; f < D / 16; ++f) *reinterpret_cast<frag_t<T> *>(ktile + TL::at(kappa(col), 2 * f + half)) = kf[f];
+  }
   const bool biased = p.bk.n > 0;
   const float scale2 = p.scale * LOG2E;
   const int nblocks = (p.nq + 31) / 32, ntiles = (p.nq + QT - 1) / QT;
@@ -669,7 +684,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D < 128 ? 2 : 1) void re
     fill.finish(bias, p.bk, p.table, p.h, head, tid, NT);
     const T *qb = reinterpret_cast<const T *>(p.q) + b * p.q_b + head * p.q_h;
     const T *gb = reinterpret_cast<const T *>(p.grad) + b * p.grad_b + head * p.grad_h;
-    const long stat = ((long)b * p.h + head) * p.nq;
+    const float2 *stats_of = p.stat + ((long)b * p.h + head) * p.nq;
+    const int2 *rows_of = p.rows + (long)b * p.nq;
     for (int chunk = tile0; chunk < tile1; chunk += 256) {
       // query tiles that see any of these keys, in order; bit 30: some query does not see all of them
       __syncthreads();
@@ -697,28 +713,25 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D < 128 ? 2 : 1) void re
       __syncthreads();
       const int n = ntodo;
       Stage<T, D, QT, NT> qs, gs;
-      float st = 0.f, dl = 0.f;
-      int rlo = 0, rhi = 0;
+      float2 st;
+      int2 row;
       auto fetch = [&](int tile) {
         const int q0 = tile * QT;
         qs.load(qb, p.q_n, q0, 0, p.nq, tid);
         gs.load(gb, p.grad_n, q0, 0, p.nq, tid);
-        if (tid < QT) {
-          const int qi = q0 + tid;
-          st = INFINITY; dl = 0.f; rlo = rhi = 0;
-          if (qi < p.nq) {
-            st = p.lse[stat + qi] - (narrow<T>() ? P_UP : 0);
-            dl = p.delta[stat + qi] * ds_factor;
-            interval(p, b, qi, rlo, rhi);
-          }
-        }
+        const int qi = min(q0 + tid % QT, p.nq - 1);       // (nothing is done to what is loaded: that would wait for the tile)
+        st = stats_of[qi];
+        row = rows_of[qi];
       };
       auto put = [&](int buf, int tile) {
         qs.store(lds + buf * 2 * TB, tile * QT, 0, p.nq, tid);
         gs.store(lds + buf * 2 * TB + TB, tile * QT, 0, p.nq, tid);
         if (tid < QT) {
-          stats[buf][0][tid] = st; stats[buf][1][tid] = dl;
-          rows[buf][0][tid] = rlo; rows[buf][1][tid] = rhi - rlo;
+          const bool some = tile * QT + tid < p.nq;
+          stats[buf][0][tid] = some ? st.x - (narrow<T>() ? P_UP : 0) : INFINITY;
+          stats[buf][1][tid] = some ? st.y * ds_factor : 0.f;
+          rows[buf][0][tid] = row.x;
+          rows[buf][1][tid] = some ? row.y : 0;
         }
       };
       if (n > 0) {
@@ -737,7 +750,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && D < 128 ? 2 : 1) void re
           f32x16 s{}, dp{};
 #pragma unroll
           for (int f = 0; f < D / 16; ++f) {
-            s = mma32(TL::row_frag(qt, u * 32 + kappa(col), 2 * f + half), kf[f], s);
+            s = mma32(TL::row_frag(qt, u * 32 + kappa(col), 2 * f + half), KL ? TL::row_frag(ktile, kappa(col), 2 * f + half) : kf[f], s);
             dp = mma32(TL::row_frag(gt, u * 32 + kappa(col), 2 * f + half), vf[f], dp);
           }
           const int p0 = q0 + u * 32 + p.offset;
@@ -853,9 +866,10 @@ Params params(const sig3d_rel_attention_args *a) {
 
 int key_splits(const sig3d_rel_attention_args *a);
 
-// workspace of the backward pass: delta (b h nq), interval summaries (b, 4 per 128 queries) int4, exponents of |dO| (f16),
-// partial table gradients
-long work_delta(const sig3d_rel_attention_args *a) { return ((long)a->b * a->h * a->nq + 3) / 4 * 4; }
+// workspace of the backward pass: lse and delta (b h nq), intervals (b nq), their summaries (b, 4 per 128 queries) int4, exponents of
+// |dO| (f16), partial table gradients
+long work_stat(const sig3d_rel_attention_args *a) { return ((long)a->b * a->h * a->nq * 2 + 3) / 4 * 4; }
+long work_rows(const sig3d_rel_attention_args *a) { return ((long)a->b * a->nq * 2 + 3) / 4 * 4; }
 long work_blocks(const sig3d_rel_attention_args *a) { return (long)a->b * sig3d_ceil_div(a->nq, NW * 32) * NW * 4; }
 long work_tops(const sig3d_rel_attention_args *a) {
   return a->dtype == 2 ? ((long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * NW + 3) / 4 * 4 : 0;
@@ -884,7 +898,7 @@ long work_ml(const sig3d_rel_attention_args *a) {
 // Splits of the dK / dV kernel.  Causal and packed rows make workgroups very unequal -- the first keys of a document are seen by
 // all of it -- so there should be several for every CU (4 for each of 256); a run of queries is worth a workgroup from 8 tiles
 // on.  A split costs a write and a read of 8 bytes an element of dK and dV.  (2 x 4096 packed tokens, 16 heads on 4, 128 wide:
-// 524 us as 256 workgroups.)
+// 524 us as 256 workgroups, at the time 245 so.)
 struct Splits { int heads, queries; };
 Splits splits_of(const sig3d_rel_attention_args *a) {
   const long base = (long)a->b * a->hkv * sig3d_ceil_div(a->nk, NW * 32);
@@ -918,7 +932,7 @@ template <typename T, int D, bool KEEP> int launch_fwd(const Params &p, hipStrea
 template <typename T, int D> int launch_bwd(const Params &p, hipStream_t stream) {
   static sig3d_once_per_device once_q, once_kv;
   const int span = (bias_floats(p.bk.reach) + 3) / 4 * 4;
-  const size_t tiles = 4 * dkv_tile<T>(D) * Tile<T, D>::ROW;
+  const size_t tiles = (4 * dkv_tile<T>(D) + (dkv_keys_in_lds<T>(D) ? NW * 32 : 0)) * Tile<T, D>::ROW;
   const size_t dq_tiles = 4 * dq_tile<T>(D) * Tile<T, D>::ROW;
   if (int e = allow_lds(rel_bwd_dq_kernel<T, D, NW>, once_q)) return e;
   if (int e = allow_lds(rel_bwd_dkv_kernel<T, D, NW>, once_kv)) return e;
@@ -971,7 +985,7 @@ extern "C" long sig3d_rel_attention_fwd_work_floats(const sig3d_rel_attention_ar
 
 extern "C" long sig3d_rel_attention_bwd_work_floats(const sig3d_rel_attention_args *a) {
   if (check("sig3d_rel_attention_bwd_work_floats", a)) return -1;
-  return work_delta(a) + work_blocks(a) + work_tops(a) + (work_hist(a) + 3) / 4 * 4 + work_part(a) + work_piece(a);
+  return work_stat(a) + work_rows(a) + work_blocks(a) + work_tops(a) + (work_hist(a) + 3) / 4 * 4 + work_part(a) + work_piece(a);
 }
 
 extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *stream) {
@@ -985,10 +999,11 @@ extern "C" int sig3d_rel_attention_bwd(const sig3d_rel_attention_args *a, void *
                 "strides must be non-negative multiples of 16 bytes, that of a token below 16 MB");
   SIG3D_REQUIRE(a->buckets.n == 0 || a->dtable, "a bias needs dtable");
   Params p = params(a);
-  p.delta = a->work;
-  p.blocks = reinterpret_cast<int4 *>(a->work + work_delta(a));
-  p.tops = reinterpret_cast<int *>(a->work + work_delta(a) + work_blocks(a));
-  p.hist = a->work + work_delta(a) + work_blocks(a) + work_tops(a);
+  p.stat = reinterpret_cast<float2 *>(a->work);
+  p.rows = reinterpret_cast<int2 *>(a->work + work_stat(a));
+  p.blocks = reinterpret_cast<int4 *>(a->work + work_stat(a) + work_rows(a));
+  p.tops = reinterpret_cast<int *>(a->work + work_stat(a) + work_rows(a) + work_blocks(a));
+  p.hist = a->work + work_stat(a) + work_rows(a) + work_blocks(a) + work_tops(a);
   const Splits s = splits_of(a);
   p.head_splits = s.heads;
   p.query_splits = s.queries;
