@@ -211,7 +211,8 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   frag_t<T> qf[NB][KS];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const int r = r0 + 16 * n + col, sub = shared ? r / per : 0, in = r - sub * per, seq = shared ? unit * p.each + sub : unit;
+    const int r = r0 + 16 * n + col, row = min(r, rows - 1);
+    const int sub = shared ? row / per : 0, in = row - sub * per, seq = shared ? unit * p.each + sub : unit;
     qhead[n] = p.t == 1 ? in : in / p.t;
     const int j = in - qhead[n] * p.t;
     pos[n] = -1;
@@ -221,12 +222,9 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
       if (j < count) pos[n] = max(len - count + j, -1);
     }
 #pragma unroll
-    for (int f = 0; f < KS; ++f) {
-      qf[n][f] = frag_t<T>{};
-      if (pos[n] >= 0)
-        qf[n][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.q) + seq * p.q_b + (long)j * p.q_n +
-                                                       (kvh * p.group + qhead[n]) * p.q_h + element<D, Q>(f, g));
-    }
+    for (int f = 0; f < KS; ++f)             // whatever stands where no query is stays in that lane's column, which `live` clears
+      qf[n][f] = *reinterpret_cast<const frag_t<T> *>(reinterpret_cast<const T *>(p.q) + seq * p.q_b + (long)j * p.q_n +
+                                                     (kvh * p.group + qhead[n]) * p.q_h + element<D, Q>(f, g));
   }
   if (biased) {
     if (tid < biases) bias[tid] = first_bias;

@@ -510,6 +510,21 @@ def test_a_captured_decoding_step_replays():
         assert caches[0].lengths.tolist() == [i + 1] * b == caches[1].lengths.tolist()
 
 
+@pytest.mark.parametrize("groups", [0, 1, 3])
+def test_queries_that_are_none_may_hold_anything(groups):
+    lang = _lang()
+    g = torch.Generator().manual_seed(12)
+    cache = _filled(g, 6, 400, 2, 64, torch.bfloat16, False, (400, 3, 17, 0, 1, 90))
+    shared = _filled(g, groups, 500, 2, 64, torch.bfloat16, False, (500, 0, 33)[:groups]) if groups else None
+    q, table, counts = _randn(g, 6, 3, 8, 64, dtype=torch.bfloat16), _randn(g, 32, 8, dtype=torch.bfloat16), _i32(3, 0, 2, 1, 3, 1)
+    want = lang.decode_attention(q, cache, shared, table, counts=counts)
+    for i, n in enumerate(counts.tolist()):
+        q[i, n:] = math.nan
+        assert not want[i, n:].any()
+    assert want.isfinite().all()
+    assert torch.equal(lang.decode_attention(q, cache, shared, table, counts=counts), want)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
 def test_many_heads_with_a_far_reach_over_shared_rows(dtype):
     """The biases of 32 query rows of as many heads would not fit into LDS."""
