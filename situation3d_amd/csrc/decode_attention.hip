@@ -11,6 +11,9 @@
 // S^T = K Q^T on 16x16x32: the K fragment is loaded straight from memory (a lane's 16 bytes are a fragment), in the row order
 // that makes two S tiles' registers the P fragment (key 8 g + 4 t + r for tile t, lane group g, register r).  V is staged in
 // wave-private LDS for the transposing read.  The next tile's loads are in flight while one is used.
+// In 16 bits a wave with one block of rows puts P into its product as two parts, rounded and rest: it waits for memory anyway (64
+// questions on a scene of 5000 rows, 30 000-token contexts: within 2 %), and the result is left with its own rounding.  Two blocks
+// would pay for it (2 scenes, 48 questions: 57 us instead of 54), for a factor of 1.4 in the error of the shared rows' part.
 // An e4m3 cache is widened to the query's type on the way in -- exact, the scale being a power of two.
 #include "lang_core.h"
 
@@ -150,6 +153,7 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
   typedef Tile<T, D, true> TL;
   typedef Flight<T, D, Q> FL;
   constexpr int KS = FL::KS, TB = KT * TL::ROW, DT = D / 16;
+  constexpr bool TWO = sizeof(T) == 2 && NB == 1;           // parts of P (see the top)
   // tiles a step: a lone wave has nobody to hide its latencies behind but its own second tile
   constexpr int NT = WV == 1 ? TILES<T, D> : 1;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
@@ -278,7 +282,7 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
 #pragma unroll
     for (int u = 0; u < NT; ++u)
       if (tile + (NT + u) * WV < to) fetch(fl[u], tile + (NT + u) * WV);
-    frag_t<T> pf[NB][NT];
+    frag_t<T> pf[NB][NT], rest[NB][TWO ? NT : 1];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       float x[8 * NT];
@@ -316,6 +320,11 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
           l[n] += e[j];
         }
         pf[n][u] = to_frag<T>(e);
+        if constexpr (TWO) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] -= (float)pf[n][u][j];
+          rest[n][u] = to_frag<T>(e);
+        }
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -325,7 +334,10 @@ __device__ __forceinline__ void walk(const DecodeParams &p, int item, bool share
       for (int u = 0; u < NT; ++u) {
         const frag_t<T> vf = TL::col_frag(vt + u * TB, 8 * g, 16 * d, lane);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) o[n][d] = mma16(vf, pf[n][u], o[n][d]);
+        for (int n = 0; n < NB; ++n) {
+          o[n][d] = mma16(vf, pf[n][u], o[n][d]);
+          if constexpr (TWO) o[n][d] = mma16(vf, rest[n][u], o[n][d]);
+        }
       }
     __builtin_amdgcn_wave_barrier();
   }

@@ -169,11 +169,12 @@ __device__ __forceinline__ Where where(int k0, int n, int p0, int reach) {
 // A wave owns 32 queries (columns), a workgroup NW waves that share the streamed key tiles in a double-buffered LDS pair:
 // the next tile's loads are in flight while the current one is used, one barrier a tile.
 // S^T = K Q^T, then O^T = V^T P^T: a query is one lane (and lane ^ 32), its softmax is in-lane work.
-// KEEP: for a backward pass to come.  The unrounded output's use is delta, and a row of dS sums to 0 only as far as delta agrees
-// with the P of the backward pass, which is not rounded: so P goes into the product as the sum of two 16-bit parts.  (With one,
-// the table's gradient of 4 x 432 bf16 tokens, 32 heads, was off by 0.0027 of its size, most of it in the buckets that hold
-// most of a row; the rounding of the result itself is 0.0017.)
-template <typename T, int D, int NW, bool KEEP>
+// TWO: 16-bit P goes into its product as the sum of two parts, rounded and rest.  Where a backward pass follows: the unrounded
+// output's use is delta, and a row of dS sums to 0 only as far as delta agrees with the P of the backward pass, which is not
+// rounded (with one part the table's gradient of 4 x 432 bf16 tokens, 32 heads, was off by 0.0027 of its size, most of it in the
+// buckets that hold most of a row; the rounding of the result itself is 0.0017).  And where the launch is small enough for latency
+// to decide (see launch_fwd).
+template <typename T, int D, int NW, bool TWO>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? (D == 128 ? 1 : 2) : D == 64 ? 3 : 2) void rel_fwd_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int KT = key_tile<T>(), NT = NW * 64, SUB = KT / 32, TB = KT * TL::ROW;
@@ -306,7 +307,6 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? (D == 128 ? 1 : 2) : D ==
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = s[u][8 * g + j];
           const frag_t<T> pf = to_frag<T>(x);
-          constexpr bool TWO = KEEP && sizeof(T) == 2;
           frag_t<T> rest;
           if constexpr (TWO) {
 #pragma unroll
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? (D == 128 ? 1 : 2) : D ==
     return;
   }
   store_row<T, D>(reinterpret_cast<T *>(p.out) + row, o, inv, half);
-  if (KEEP) {
+  if (p.out32) {
     store_row<float, D>(p.out32 + row, o, inv, half);
     if (half == 0) p.lse[((long)b * p.h + head) * p.nq + qi] = empty ? INFINITY : m + __builtin_amdgcn_logf(l);
   }
@@ -916,11 +916,11 @@ long work_part(const sig3d_rel_attention_args *a) {
   return n > 1 ? 2 * n * a->b * a->nk * a->hkv * a->d : 0;
 }
 
-template <typename T, int D, bool KEEP> int launch_fwd(const Params &p, hipStream_t stream) {
+template <typename T, int D, bool TWO> int launch_fwd(const Params &p, hipStream_t stream) {
   static sig3d_once_per_device once;
   const size_t lds = 4 * key_tile<T>() * Tile<T, D>::ROW + bias_floats(p.bk.reach) * sizeof(float);
-  if (int e = allow_lds(rel_fwd_kernel<T, D, NW, KEEP>, once)) return e;
-  rel_fwd_kernel<T, D, NW, KEEP><<<p.b * p.h * p.qtiles * p.key_splits, NW * 64, lds, stream>>>(p);
+  if (int e = allow_lds(rel_fwd_kernel<T, D, NW, TWO>, once)) return e;
+  rel_fwd_kernel<T, D, NW, TWO><<<p.b * p.h * p.qtiles * p.key_splits, NW * 64, lds, stream>>>(p);
   SIG3D_LAUNCH_CHECK("rel_fwd_kernel");
   if (p.piece) {
     rel_join_kernel<T, D><<<sig3d_ceil_div((long)p.b * p.nq * p.h, 256 / (D / 4)), 256, 0, stream>>>(p);
@@ -974,7 +974,12 @@ extern "C" int sig3d_rel_attention_fwd(const sig3d_rel_attention_args *a, void *
   return by_type(a->dtype, a->d, [&](auto t, auto d) {
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
-    return p.out32 ? launch_fwd<T, D, true>(p, (hipStream_t)stream) : launch_fwd<T, D, false>(p, (hipStream_t)stream);
+    // P in two parts (see the kernel) without a backward pass: up to one workgroup for each of 256 CUs.  (12 heads of 52 bf16
+    // tokens: 8.2 us instead of 7.8; 16 heads of 200: 12.3 instead of 11.6; 512 workgroups, 128 heads of 432: 25.7 instead of 22.1.)
+    if constexpr (sizeof(T) == 2) {
+      if (p.out32 || (long)p.b * p.h * p.qtiles * p.key_splits <= 256) return launch_fwd<T, D, true>(p, (hipStream_t)stream);
+    }
+    return launch_fwd<T, D, false>(p, (hipStream_t)stream);
   });
 }
 
