@@ -15,7 +15,10 @@
 // an operand of the next product (bf16 / f16 matrix instructions take nothing else; f32 stays f32).  f16 has no exponents to
 // spare for that -- P is 1 / nk on average, gradients are small -- so its backward pass holds 2^8 P and dS times the power of
 // two that brings the largest |dO| (of the query for dQ, of the sequence's queries for dK) to [4, 8), and takes both back out
-// of the f32 sums.
+// of the f32 sums.  |dS| may be as large as 2 |dO|_1 max |V|: where that power is too much for f16 (65504) it is lowered.  For dQ
+// when a block's dS reaches DS_MOST -- like the running maximum, a branch seldom taken (16 heads of 128 on 4, 2 x 4096 packed
+// tokens: 156 us without it, 158 with it); for dK beforehand, by the largest |dS| that the dQ kernel has met (a branch there as
+// well: 245 us instead of 200).
 #include "lang_core.h"
 
 #include <limits.h>
@@ -35,7 +38,7 @@ struct Params {
   float *part;                                // backward: dK, dV of every split, (2, splits, b, nk, hkv, d), or NULL: one split
   float *piece, *piece_ml;                    // one output, maximum and sum (forward), one dQ for every key split, or NULL
   int4 *blocks;                               // backward: interval summary of every 32 queries
-  int *tops;                                  // backward, f16: exponent of the largest |dO| of a head's 32 queries
+  int *tops;                                  // backward, f16: by how much a head's 32 queries let dS be raised for dK (see dQ)
   long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, grad_b, grad_n, grad_h;
   int b, nq, nk, h, hkv, group, causal, offset, table_rows, qtiles, ktiles, head_splits, query_splits, key_splits;
   float scale;
@@ -140,6 +143,15 @@ __device__ __forceinline__ void store_row(T *row, const f32x16 (&acc)[D / 32], f
 template <typename T> constexpr bool narrow() { return std::is_same<T, _Float16>::value; }
 constexpr float SLACK = 8.f;                  // of the forward pass's reference value (see there)
 constexpr int P_UP = 8, DS_UP = 3;            // f16: exponents that P and dS are raised by (see the top)
+// f16: from DS_MOST on, a query's dS is brought back to [2^(DS_KEEP - 1), 2^DS_KEEP): half a subnormal step is then at most 2^-36
+// of its largest.  For dK the largest of all is below 2^DS_TOP (dP and delta are summed in another order there: an error of 2^9 at
+// most where |dO| < 8, |V| <= 65504 and d = 128, which 65504 still holds).
+constexpr float DS_MOST = 32768.f;
+constexpr int DS_KEEP = 12, DS_TOP = 14;
+// exponents by which dS of a query whose largest one is `top` has to go down (an infinite one stays where it is)
+__device__ __forceinline__ int too_much(float top) {
+  return top >= DS_MOST && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - DS_KEEP : 0;
+}
 
 template <typename T> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
 // keys of a tile of the dQ kernel: 32 leave LDS and registers for two workgroups a CU where a row is long
@@ -452,6 +464,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
   }
   if (!valid) lse = INFINITY;
   float undo = 1.f;                                       // dS is held times 1 / undo
+  float peak = 0.f;                                       // f16: the largest |dS|, as held
+  int grads = -64;                                        // f16: exponent of the largest |dO|; -64: none
   if constexpr (narrow<T>()) {
     float top = 0.f;
 #pragma unroll
@@ -463,8 +477,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
     const int e = plain ? DS_UP : __builtin_amdgcn_frexp_expf(top);      // top in [2^(e-1), 2^e)
     undo = __builtin_ldexpf(1.f, e - DS_UP);
     lse += (float)(e - DS_UP);
-    const int most = wave_max_i32(plain ? -64 : e);
-    if (lane == 0 && split == 0) p.tops[((long)bh * p.qtiles + qt) * NW + wave] = most;
+    if (!plain) grads = e;
   }
   const bool biased = p.bk.n > 0;
   if (biased) {
@@ -521,6 +534,25 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
           for (int r = 0; r < 16; ++r)
             if ((unsigned)(t + u * 32 + reg_row(r, half) - lo) >= (unsigned)(hi - lo)) s[r] = 0.f;
         }
+        if constexpr (narrow<T>()) {
+          float top = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[r]));
+          peak = fmaxf(peak, top);
+          if (__any(top >= DS_MOST)) {
+            const int down = too_much(max_halves(top));
+            const float keep = __builtin_ldexpf(1.f, -down);
+            peak *= keep;
+            undo = __builtin_ldexpf(undo, down);
+            lse += (float)down;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= keep;
+#pragma unroll
+            for (int blk = 0; blk < D / 32; ++blk)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) dq[blk][r] *= keep;
+          }
+        }
         if (biased) {
           if (w == NEAR) {
 #pragma unroll
@@ -560,6 +592,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
       vs.store(lds + (buf ^ 1) * 2 * TB + TB, t + KT, wlo, whi, tid);
     }
     __syncthreads();
+  }
+  if constexpr (narrow<T>()) {
+    peak *= undo;
+    if (peak > 0.f && peak < INFINITY && grads > -64) grads = max(grads, __builtin_amdgcn_frexp_expf(peak) - (DS_TOP - DS_UP));
+    const int most = wave_max_i32(grads);
+    if (lane == 0) p.tops[(((long)bh * p.qtiles + qt) * NW + wave) * p.key_splits + split] = most;
   }
   if (valid) {
     if (p.piece) store_row<float, D>(p.piece + split * ((long)p.b * p.nq * p.h * D) + row, dq, p.scale * undo, half);
@@ -662,9 +700,10 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 ? D < 128 : D == 64) ? 2 :
   int up = 0;                                  // f16: dS is held times 2^up, P times 2^P_UP
   if constexpr (narrow<T>()) {
     int most = -64;
-    for (int i = tid; i < p.group * nblocks; i += NT) {
-      const int hh = i / nblocks, blk = i - hh * nblocks;
-      most = max(most, p.tops[((long)b * p.h + kvh * p.group + hh) * p.qtiles * NW + blk]);
+    const int each = nblocks * p.key_splits;
+    for (int i = tid; i < p.group * each; i += NT) {
+      const int hh = i / each;
+      most = max(most, p.tops[((long)b * p.h + kvh * p.group + hh) * p.qtiles * NW * p.key_splits + (i - hh * each)]);
     }
     most = wave_max_i32(most);
     if (lane == 0) todo[wave] = most;
@@ -867,13 +906,13 @@ Params params(const sig3d_rel_attention_args *a) {
 
 int key_splits(const sig3d_rel_attention_args *a);
 
-// workspace of the backward pass: lse and delta (b h nq), intervals (b nq), their summaries (b, 4 per 128 queries) int4, exponents of
-// |dO| (f16), partial table gradients
+// workspace of the backward pass: lse and delta (b h nq), intervals (b nq), their summaries (b, 4 per 128 queries) int4, exponents
+// (f16), partial table gradients
 long work_stat(const sig3d_rel_attention_args *a) { return ((long)a->b * a->h * a->nq * 2 + 3) / 4 * 4; }
 long work_rows(const sig3d_rel_attention_args *a) { return ((long)a->b * a->nq * 2 + 3) / 4 * 4; }
 long work_blocks(const sig3d_rel_attention_args *a) { return (long)a->b * sig3d_ceil_div(a->nq, NW * 32) * NW * 4; }
 long work_tops(const sig3d_rel_attention_args *a) {
-  return a->dtype == 2 ? ((long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * NW + 3) / 4 * 4 : 0;
+  return a->dtype == 2 ? ((long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * NW * key_splits(a) + 3) / 4 * 4 : 0;
 }
 long work_hist(const sig3d_rel_attention_args *a) {
   return a->buckets.n > 0 ? (long)a->b * a->h * sig3d_ceil_div(a->nq, NW * 32) * key_splits(a) * a->table_rows : 0;

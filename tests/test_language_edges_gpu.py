@@ -1,0 +1,120 @@
+"""Language-side operators on the GPU: f16 gradients of values of very different size."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import language_ref as ref  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+NAMES = ("dq", "dk", "dv", "dtable")
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _randn(g, *shape, dtype=torch.float32):
+    return torch.randn(shape, generator=g).to(dtype).to(DEV)
+
+
+def _lang():
+    from situation3d_amd import language
+    return language
+
+
+# ---- f16: dS beyond what f16 holds -----------------------------------------------------------------------------------------
+
+def _ds_most(q, k, v, table, grad, ok, scale, index):
+    """max |dS| over all pairs."""
+    q, k, v, do = (x.detach().double().cpu().transpose(1, 2) for x in (q, k, v, grad))
+    group = q.shape[1] // k.shape[1]
+    k, v = (x.repeat_interleave(group, 1) for x in (k, v))
+    s = scale * q @ k.transpose(2, 3)
+    if table is not None:
+        s = s + table.detach().double().cpu()[index].permute(2, 0, 1)
+    s = s.masked_fill(~ok[:, None], -torch.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)
+    dp = do @ v.transpose(2, 3)
+    return float((p * (dp - (p * dp).sum(-1, keepdim=True))).abs().max())
+
+
+def _check_large(q, k, v, table, grad, ok, index, opts, scale):
+    """language_ref's bounds, and what lowering the exponent costs: dS is then held times a power of two that keeps the largest of
+    a query (dQ) or key (dK) at 2^11 or more, so that half a subnormal step of f16, 2^-25, stands for at most 2^-36 max |dS|."""
+    want = ref.attention(q, k, v, table, ok, scale, index, grad)
+    group = q.shape[2] // k.shape[2]
+    most = _ds_most(q, k, v, table, grad, ok, scale, index) * 2.0 ** -36
+    seen = ok[:, None].double()
+    kk = k.double().abs().cpu().transpose(1, 2).repeat_interleave(group, 1)
+    more_q = (scale * most * seen @ kk).transpose(1, 2)
+    more_k = scale * most * seen.transpose(2, 3) @ q.double().abs().cpu().transpose(1, 2)
+    more_k = more_k.view(k.shape[0], k.shape[2], group, k.shape[1], k.shape[3]).sum(2).transpose(1, 2)
+    want["dq"] = want["dq"][0], want["dq"][1] + more_q
+    want["dk"] = want["dk"][0], want["dk"][1] + more_k
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, table) if x is not None]
+    out = _lang().relative_attention(*leaves, **opts)
+    ref.check("out", out, want["out"])
+    for name, x in zip(NAMES, torch.autograd.grad(out, leaves, grad)):
+        ref.check(name, x, want[name])
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_f16_gradients_of_two_large_opposite_values(d):
+    """dS = +-dO d V / 2 = +-128 for d = 128: more than f16 holds once dO = 0.01 has been raised to 4."""
+    q, k = torch.zeros(1, 1, 1, d, dtype=torch.float16, device=DEV), torch.ones(1, 2, 1, d, dtype=torch.float16, device=DEV)
+    k[0, 1] = -1
+    q[..., 0] = 1
+    k[..., 0] = 0.5                                   # the scores are equal, dQ is not 0
+    v = torch.full((1, 2, 1, d), 200.0, dtype=torch.float16, device=DEV)
+    v[0, 1] = -200
+    grad = torch.full((1, 1, 1, d), 0.01, dtype=torch.float16, device=DEV)
+    _check_large(q, k, v, None, grad, ref.seen(1, 1, 2), None, {}, d ** -0.5)
+
+
+# b, nq, nk, h, hkv, d, options: one tile; several, causal; runs of keys; runs of queries
+LARGE = [(2, 40, 60, 2, 1, 64, dict(key_lengths=(60, 33))), (1, 200, 200, 4, 2, 128, dict(causal=True, bidirectional=False)),
+         (1, 70, 1100, 2, 2, 96, {}), (1, 1100, 150, 4, 1, 64, {}), (2, 300, 300, 2, 2, 96, dict(causal=True))]
+
+
+@pytest.mark.parametrize("n", range(len(LARGE)))
+@pytest.mark.parametrize("where", ["all", "late", "one"])
+def test_f16_gradients_where_v_is_large_and_grads_are_small(n, where):
+    """V of many thousand: everywhere, in late keys alone (the exponent moves between tiles), in one row; dO of many sizes.  Raised to
+    4 <= max |dO| < 8, dS reaches 70 000 to 340 000 for dQ in all of these but one, up to 175 000 for dK."""
+    b, nq, nk, h, hkv, d, opts = LARGE[n]
+    opts = dict(opts)
+    g = torch.Generator().manual_seed(n)
+    f16 = torch.float16
+    q, k, table = _randn(g, b, nq, h, d, dtype=f16) * 4, _randn(g, b, nk, hkv, d, dtype=f16), _randn(g, 32, h, dtype=f16)
+    v = _randn(g, b, nk, hkv, d)
+    if where == "all":
+        v *= 12000
+    elif where == "late":
+        v[:, nk * 2 // 3:] *= 12000
+    else:
+        v[:, nk // 2] *= 14000
+    # sizes 2^-16 .. 2^-8 by query: dQ and dK stay below 65504
+    grad = _randn(g, b, nq, h, d) * torch.exp2(-8 - 8 * torch.rand(b, nq, 1, 1, generator=g)).to(DEV)
+    if "key_lengths" in opts:
+        opts["key_lengths"] = _i32(*opts["key_lengths"])
+    ok = ref.seen(b, nq, nk, opts.get("causal", False), 0, opts.get("key_lengths"))
+    index = ref.bucket_matrix(nq, nk, 0, 32, 128, opts.get("bidirectional", True))
+    _check_large(q, k, v.to(f16), table, grad.to(f16), ok, index, opts, d ** -0.5)
+
+
+def test_f16_infinite_grads_stay_where_they_are():
+    """An infinite dO makes its own query's dQ and what it touches infinite or NaN, and nothing else (dV^T = dO^T P: its own element of
+    every key's dV, 0 times infinity for the keys that it does not see)."""
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (_randn(g, 1, 100, 2, 64, dtype=torch.float16).requires_grad_() for _ in range(3))
+    grad = _randn(g, 1, 100, 2, 64, dtype=torch.float16)
+    grad[0, 50, 1, 7] = torch.inf
+    dq, dk, dv = torch.autograd.grad(_lang().relative_attention(q, k, v, causal=True), (q, k, v), grad)
+    assert dq[0, :, 0].isfinite().all() and dk[0, :, 0].isfinite().all() and dv[0, :, 0].isfinite().all()
+    assert not dq[0, 50, 1].isfinite().any()
+    others, rest = torch.arange(100, device=DEV) != 50, torch.arange(64, device=DEV) != 7
+    assert dq[0, others, 1].isfinite().all() and dk[0, 51:, 1].isfinite().all() and dv[0, :, 1, rest].isfinite().all()
