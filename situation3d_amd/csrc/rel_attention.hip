@@ -14,7 +14,7 @@
 // Statistics, accumulators, the running maximum and sum are f32.  P and dS are rounded to the operand type where they become
 // an operand of the next product (bf16 / f16 matrix instructions take nothing else; f32 stays f32).  f16 has no exponents to
 // spare for that -- P is 1 / nk on average, gradients are small -- so its backward pass holds 2^8 P and dS times the power of
-// two that brings the largest |dO| (of the query for dQ, of the sequence's queries for dK) to [4, 8), and takes both back out
+// two that brings the largest |dO| (of the query for dQ, of the queries that see a key for dK) to [4, 8), and takes both back out
 // of the f32 sums.  |dS| may be as large as 2 |dO|_1 max |V|: where that power is too much for f16 (65504) it is lowered.  For dQ
 // when a block's dS reaches DS_MOST -- like the running maximum, a branch seldom taken (16 heads of 128 on 4, 2 x 4096 packed
 // tokens: 156 us without it, 158 with it); for dK beforehand, by the largest |dS| that the dQ kernel has met (a branch there as
@@ -476,8 +476,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 ? 1 : 2) void rel_bwd_dq_ke
     const bool plain = !(top > 0.f && top < INFINITY);
     const int e = plain ? DS_UP : __builtin_amdgcn_frexp_expf(top);      // top in [2^(e-1), 2^e)
     undo = __builtin_ldexpf(1.f, e - DS_UP);
+    if (!plain && lse < INFINITY) grads = e;              // (a query that sees nothing has no gradient, whatever its dO is)
     lse += (float)(e - DS_UP);
-    if (!plain) grads = e;
   }
   const bool biased = p.bk.n > 0;
   if (biased) {

@@ -118,3 +118,35 @@ def test_f16_infinite_grads_stay_where_they_are():
     assert not dq[0, 50, 1].isfinite().any()
     others, rest = torch.arange(100, device=DEV) != 50, torch.arange(64, device=DEV) != 7
     assert dq[0, others, 1].isfinite().all() and dk[0, 51:, 1].isfinite().all() and dv[0, :, 1, rest].isfinite().all()
+
+
+# ---- f16: grads of queries that see nothing -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("how", ["masked", "biased"])
+def test_f16_grads_of_queries_that_see_nothing_decide_nothing(how):
+    """Their dO passes no gradient, so neither does its size decide how dS of the others is held."""
+    g = torch.Generator().manual_seed(4)
+    f16 = torch.float16
+    q, k, v = (_randn(g, 1, 90, 2, 64, dtype=f16) for _ in range(3))
+    table = _randn(g, 32, 2, dtype=f16)
+    grad = _randn(g, 1, 90, 2, 64, dtype=f16) * 2.0 ** -10
+    index = ref.bucket_matrix(90, 90, 0, 32, 128, True)
+    if how == "masked":
+        r = torch.tensor([0, 90]).repeat(1, 90, 1).int()
+        r[0, 30:60] = 0
+        opts, ok = dict(key_ranges=r.to(DEV)), ref.seen(1, 90, 90, key_ranges=r)
+    else:                                             # a query whose only keys have a bias of -inf
+        r = torch.tensor([0, 90]).repeat(1, 90, 1).int()
+        r[0, 30:60, 0], r[0, 30:60, 1] = torch.arange(30, 60).int(), torch.arange(31, 61).int()
+        table[0] = -torch.inf                         # its own place
+        opts, ok = dict(key_ranges=r.to(DEV)), ref.seen(1, 90, 90, key_ranges=r) & (index != 0)
+    live = ok[0].any(1)
+    assert not live[30:60].any() and live[:30].all() and live[60:].all()
+    held = torch.where(live.to(DEV)[None, :, None, None], grad, 0.0)
+    want = ref.attention(q, k, v, torch.where(table.isinf(), 0.0, table), ok, 0.125, index, held)
+    grad[0, 30:60] = 30000
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, table)]
+    out = _lang().relative_attention(*leaves, **opts)
+    ref.check("out", out, want["out"])
+    for name, x in zip(NAMES, torch.autograd.grad(out, leaves, grad)):
+        ref.check(name, x, want[name])
