@@ -19,6 +19,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -115,6 +116,12 @@ def _check_table(shape, dtype, heads, q_dtype, what):
 def _no_gradient(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad()" % what)
+
+
+def _no_tangent(what, *tensors):
+    """A dual tensor does not show in requires_grad: its tangent would be dropped."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("%s has no forward-mode derivative" % what)
 
 
 def _int_array(t, shape, device, name):
@@ -219,6 +226,7 @@ class _RelativeAttentionFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _no_tangent("relative_attention's backward pass", grad)
         q, k, v, table, out32, lse, *arrays = ctx.saved_tensors
         cfg, a, work, strides = ctx.call
         dev = q.device
@@ -253,7 +261,8 @@ class _RelativeAttentionFn(torch.autograd.Function):
 
 def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, max_distance=128, causal=False, query_offset=0,
                        key_lengths=None, prefix_lengths=None, key_ranges=None):
-    """softmax(scale q k^T + bias) v over the keys that each query sees; gradients for q, k, v and table.
+    """softmax(scale q k^T + bias) v over the keys that each query sees; gradients for q, k, v and table (first derivatives in
+    reverse mode: a second one and forward mode are refused).
 
     q (b, nq, h, d), k / v (b, nk, hkv, d), hkv dividing h: head i reads key head i // (h / hkv).  Query i stands at position
     p = i + query_offset, key j at j.
@@ -272,6 +281,7 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
         raise RuntimeError("CPU not supported")
     if k.device != dev or v.device != dev or table is not None and table.device != dev:
         raise RuntimeError("all tensors must be on the same device")
+    _no_tangent("relative_attention", q, k, v, table)
     if prefix_lengths is not None and not causal:
         raise RuntimeError("relative_attention: prefix_lengths only means something with causal=True")
     cfg = (float(q.shape[-1] ** -0.5 if scale is None else scale), bool(bidirectional), int(max_distance), bool(causal),
@@ -354,6 +364,7 @@ class KVCache:
             raise RuntimeError("all tensors must be on the same device")
         if k.requires_grad or v.requires_grad:
             _no_gradient("KVCache.append", k, v)
+        _no_tangent("KVCache.append", k, v)
         shape = k.shape
         if len(shape) != 4 or v.shape != shape or shape[0] != self.batch or shape[2:] != (self.kv_heads, self.head_dim):
             raise RuntimeError("KVCache.append: k and v must be (%d, t, %d, %d)" % (self.batch, self.kv_heads, self.head_dim))
@@ -410,6 +421,7 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
         raise RuntimeError("all tensors must be on the same device")
     if q.requires_grad or table is not None and table.requires_grad:
         _no_gradient(what, q, table)
+    _no_tangent(what, q, table)
     if q.dim() != 4 or q.dtype != cache.dtype:
         raise RuntimeError("%s: q is (batch, new tokens, heads, head size) in the cache's type" % what)
     b, t, h, d = shape = q.shape

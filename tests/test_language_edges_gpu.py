@@ -1,4 +1,4 @@
-"""Language-side operators on the GPU: f16 gradients of values of very different size."""
+"""Language-side operators on the GPU: f16 gradients of values of very different size, forward-mode derivatives."""
 import os
 import sys
 
@@ -150,3 +150,35 @@ def test_f16_grads_of_queries_that_see_nothing_decide_nothing(how):
     ref.check("out", out, want["out"])
     for name, x in zip(NAMES, torch.autograd.grad(out, leaves, grad)):
         ref.check(name, x, want[name])
+
+
+# ---- forward-mode derivatives ---------------------------------------------------------------------------------------------------
+
+def test_tangents_are_refused():
+    """There are no forward-mode derivatives; a dual tensor's tangent is never dropped."""
+    from torch.autograd import forward_ad as fwd
+    lang = _lang()
+    q, k, v = (torch.randn(2, 5, 2, 64, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    table = torch.randn(32, 2, device=DEV, dtype=torch.bfloat16)
+    ranges = _i32(*[0, 5] * 10).view(2, 5, 2)
+    cache = lang.KVCache(2, 8, 2, 64, torch.bfloat16, False, DEV)
+    cache.append(k, v)
+    calls = [(lambda q, k, v, t: lang.relative_attention(q, k, v, t), 4), (lambda q, k, v, t: cache.append(k, v, start=_i32(0, 0)), (1, 2)),
+             (lambda q, k, v, t: lang.decode_attention(q, cache, None, t), (0, 3)),
+             (lambda q, k, v, t: lang.relative_attention(q[:, :, :, :], k, v, t, key_ranges=ranges), 4)]
+    with fwd.dual_level():
+        for call, which in calls:
+            args = [q, k, v, table]
+            call(*args)                                # nothing dual: as ever
+            for i in range(4) if which == 4 else which:
+                dual = [fwd.make_dual(x, torch.ones_like(x)) if j == i else x for j, x in enumerate(args)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+        leaf = q.clone().requires_grad_()
+        out = lang.relative_attention(leaf, k, v, table)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, leaf, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: lang.relative_attention(x, k, v, table), (q,), (torch.ones_like(q),))
