@@ -64,9 +64,10 @@ def _bucket_struct(buckets, max_distance, bidirectional):
 
 
 def _readable(shape, stride, itemsize):
-    """Rows as the kernels read them: dense, strides multiples of 16 bytes, a token's below 16 MB."""
+    """Rows as the kernels read them: dense, strides multiples of 16 bytes, a token's below 16 MB; strides of dimensions of one do
+    not matter."""
     return (stride[-1] == 1 or shape[-1] == 1) and all(n == 1 or s >= 0 and s * itemsize % 16 == 0 for n, s in
-                                                      zip(shape[:-1], stride[:-1])) and stride[1] * itemsize < 1 << 24
+                                                      zip(shape[:-1], stride[:-1])) and (shape[1] == 1 or stride[1] * itemsize < 1 << 24)
 
 
 def _strides(shape, stride):
@@ -300,7 +301,9 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
         a.key_lengths, a.prefix_lengths, a.key_ranges = (None if x is None else x.data_ptr() for x in arrays)
     if not ok:
         q, k, v = _rows(q), _rows(k), _rows(v)
-        a, _, work = _rel_args(q, k, v, table, cfg, arrays)
+        a, ok, work = _rel_args(q, k, v, table, cfg, arrays)
+        if not ok:
+            raise RuntimeError("relative_attention: a token's heads must be below 16 MB")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or table is not None and table.requires_grad):
         return _RelativeAttentionFn.apply(q, k, v, table, cfg, arrays, a, work)

@@ -1,0 +1,46 @@
+"""Language-side operators without a GPU: strides of dimensions of one."""
+import pytest
+import torch
+
+CFG = (1.0, True, 128, False, 0)
+
+
+def _template(q, k):
+    from situation3d_amd import language
+    return language._rel_template(q.shape, q.stride(), k.shape, k.stride(), k.shape, k.stride(), (q.dtype,) * 3, None, None, CFG)
+
+
+def _one(shape, stride, dtype=torch.bfloat16):
+    """`shape` over a storage of its elements: only the strides of dimensions of one are beyond it."""
+    n = 1
+    for x in shape:
+        n *= x
+    return torch.empty(n, dtype=dtype).as_strided(shape, stride)
+
+
+@pytest.mark.parametrize("stride", [(256, 1 << 23, 64, 1), (7, 1 << 40, 64, 1), (256, 3, 64, 1)], ids=str)
+@pytest.mark.parametrize("nk", [5, 2000])
+def test_the_stride_of_a_single_token_does_not_matter(stride, nk):
+    """One token sliced out of a token-major buffer: its stride is nobody's, and may be 16 MB and more."""
+    from situation3d_amd import language
+    k, dense = torch.empty(1, nk, 4, 64, dtype=torch.bfloat16), torch.empty(1, 1, 4, 64, dtype=torch.bfloat16)
+    for q, keys in ((_one((1, 1, 4, 64), stride), k), (dense, _one((1, 1, 4, 64), stride))):
+        other = torch.empty(q.shape if keys is not k else (1, 1, 4, 64), dtype=torch.bfloat16)
+        a, ok, work = _template(q, keys)
+        _, _, want = _template(other, keys if keys is k else other)
+        assert ok and work == want and a.q_n == a.q_b == 0
+    assert language._rows(_one((1, 1, 4, 64), stride)).shape == (1, 1, 4, 64)
+
+
+def test_what_cannot_be_read_is_copied():
+    from situation3d_amd import language
+    for t in (torch.empty(2, 3, 4, 65)[..., 1:], torch.empty(1, 3, 4, 64).expand(2, 3, 4, 64), torch.empty(2, 3, 64, 4).transpose(2, 3),
+              torch.empty(2, 1, 1, 64), torch.empty(3, 2, 4, 64).transpose(0, 1), torch.empty(2, 3, 4, 1).expand(2, 3, 4, 64)):
+        r = language._rows(t)
+        assert language._readable(r.shape, r.stride(), 4) and torch.equal(r.isnan(), t.isnan())
+
+
+def test_tokens_of_16_mb_are_refused():
+    """A dense tensor whose tokens are that long cannot be copied into a shape that the kernels read."""
+    q = torch.empty(1, 2, 1 << 17, 64, dtype=torch.float16, device="meta")
+    assert not _template(q, q)[1]

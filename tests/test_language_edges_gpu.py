@@ -1,4 +1,5 @@
-"""Language-side operators on the GPU: f16 gradients of values of very different size, forward-mode derivatives."""
+"""Language-side operators on the GPU: f16 gradients of values of very different size, forward-mode derivatives,
+odd strides."""
 import os
 import sys
 
@@ -182,3 +183,29 @@ def test_tangents_are_refused():
             torch.autograd.grad(out, leaf, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: lang.relative_attention(x, k, v, table), (q,), (torch.ones_like(q),))
+
+
+# ---- strides -----------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("nk", [5, 2000])
+def test_the_stride_of_a_single_token_does_not_matter(nk):
+    """One token out of a token-major buffer of 16 MB a token; with many keys the call needs a workspace."""
+    g = torch.Generator().manual_seed(6)
+    big = torch.zeros(2 * (1 << 23), dtype=torch.bfloat16, device=DEV)
+    q = big.as_strided((1, 1, 4, 64), (256, 1 << 23, 64, 1))
+    dense = _randn(g, 1, 1, 4, 64, dtype=torch.bfloat16)
+    q.copy_(dense)
+    k, v = _randn(g, 1, nk, 2, 64, dtype=torch.bfloat16), _randn(g, 1, nk, 2, 64, dtype=torch.bfloat16)
+    grads = []
+    for x in (q, dense):
+        leaves = [x.detach().requires_grad_(), k.detach().requires_grad_(), v.detach().requires_grad_()]
+        out = _lang().relative_attention(*leaves)
+        grads.append([out.detach(), *torch.autograd.grad(out, leaves, dense)])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_tokens_of_16_mb_are_refused():
+    q = torch.zeros(1, 2, 1 << 17, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(RuntimeError, match="16 MB"):
+        _lang().relative_attention(q, q, q)
+    assert not _lang().relative_attention(q[:, :1], q[:, :1], q[:, :1]).any()      # a single one has no stride
