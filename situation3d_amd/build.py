@@ -44,6 +44,10 @@ def build(force=False, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     hipcc = _hipcc()
     jobs = []
+    # the command that the objects were compiled with: others are compiled again (missing while some may be of either)
+    stamp, command = os.path.join(OBJ, "command"), " ".join([hipcc] + FLAGS)
+    if not os.path.exists(stamp) or open(stamp).read() != command:
+        force = True
     # longest compile first (measured, seconds on one core of the build container; the rest by size)
     cost = {"decode_attention.hip": 55, "shared_mlp_fwd4r.hip": 44, "rel_attention.hip": 29, "gemmp.hip": 33, "shared_mlp_fwd2.hip": 30, "gemm16.hip": 26,
             "shared_mlp_fwd4.hip": 21, "shared_mlp_fwd1.hip": 18, "shared_mlp.hip": 13}
@@ -59,9 +63,13 @@ def build(force=False, verbose=False):
         subprocess.check_call(cmd)
 
     if jobs:
+        if force and os.path.exists(stamp):
+            os.remove(stamp)
         # the longest translation unit (decode_attention.hip, ~55 s alone) bounds the wall time once every file has a core
         with ThreadPoolExecutor(max_workers=min(os.cpu_count() or 4, 8, len(jobs))) as ex:
             list(ex.map(run, jobs))
+        with open(stamp, "w") as f:
+            f.write(command)
     objs = [os.path.join(OBJ, s.replace(".hip", ".o")) for s in SOURCES]
     if force or jobs or _stale(LIB, objs):
         run([hipcc, "-shared", "-fPIC", "--offload-arch=gfx950", "-o", LIB] + objs)

@@ -1,0 +1,64 @@
+"""The build recipe without a compiler: what is compiled again, and when."""
+import os
+
+import pytest
+
+
+@pytest.fixture
+def recipe(tmp_path, monkeypatch):
+    """situation3d_amd.build over a folder of its own; run() -> the sources it compiled, and whether it linked."""
+    from situation3d_amd import build
+    monkeypatch.setattr(build, "OBJ", str(tmp_path / "obj"))
+    monkeypatch.setattr(build, "LIB", str(tmp_path / "lib.so"))
+    calls = []
+
+    def compiler(cmd):
+        calls.append(cmd)
+        if build.fail in cmd:
+            raise RuntimeError("compiler")
+        with open(cmd[cmd.index("-o") + 1], "w"):
+            pass
+
+    monkeypatch.setattr(build.subprocess, "check_call", compiler)
+    monkeypatch.setattr(build, "fail", None, raising=False)
+
+    def run(**kw):
+        calls.clear()
+        build.build(**kw)
+        return sorted(os.path.basename(c[c.index("-c") + 1]) for c in calls if "-c" in c), any("-shared" in c for c in calls)
+
+    build_run = run
+    build_run.module = build
+    return build_run
+
+
+def test_objects_of_other_flags_are_compiled_again(recipe, monkeypatch):
+    build = recipe.module
+    everything = sorted(build.SOURCES)
+    assert recipe() == (everything, True)
+    assert recipe() == ([], False)
+    monkeypatch.setattr(build, "FLAGS", build.FLAGS + ["-DOTHER"])
+    assert recipe() == (everything, True)
+    assert recipe() == ([], False)
+    monkeypatch.setenv("HIPCC", os.path.abspath(__file__))                # another compiler
+    assert recipe() == (everything, True)
+
+
+def test_an_interrupted_build_leaves_no_mixture(recipe, monkeypatch):
+    build = recipe.module
+    assert recipe()[1]
+    flags = build.FLAGS
+    monkeypatch.setattr(build, "FLAGS", flags + ["-DOTHER"])
+    monkeypatch.setattr(build, "fail", os.path.join(build.CSRC, build.SOURCES[0]))
+    with pytest.raises(RuntimeError):
+        recipe()
+    monkeypatch.setattr(build, "FLAGS", flags)
+    monkeypatch.setattr(build, "fail", None)
+    assert recipe() == (sorted(build.SOURCES), True)
+
+
+def test_objects_without_a_record_are_compiled_again(recipe):
+    build = recipe.module
+    assert recipe()[1]
+    os.remove(os.path.join(build.OBJ, "command"))
+    assert recipe() == (sorted(build.SOURCES), True)
