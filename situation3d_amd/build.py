@@ -17,9 +17,11 @@ SOURCES = ["capi.hip", "sampling.hip", "ball_query.hip", "group_points.hip", "in
            "situational.hip", "attention.hip", "shared_mlp.hip", "shared_mlp_fwd1.hip", "shared_mlp_fwd2.hip", "shared_mlp_fwd4.hip", "shared_mlp_fwd4r.hip", "pos_embed.hip", "rowops.hip", "optim.hip", "voxelize.hip", "compact.hip", "gemm16.hip", "gemmp.hip", "sqa_loss.hip", "sa_first.hip", "small_mlp.hip", "qformer_embed.hip", "heads.hip", "rel_attention.hip", "kv_cache.hip", "decode_attention.hip"]
 HEADERS = [os.path.join(CSRC, "sig3d_common.h"), os.path.join(CSRC, "shared_mlp_fwd.h"), os.path.join(CSRC, "gemm16_core.h"), os.path.join(CSRC, "gemmp_core.h"), os.path.join(CSRC, "situational_pose.h"),
            os.path.join(HERE, "..", "include", "sig3d_hip.h"), os.path.join(HERE, "..", "include", "sig3d_debug.h")]
+# headers of some sources alone
+LANG_HEADER = os.path.join(CSRC, "lang_core.h")
+HEADERS_OF = {src: [LANG_HEADER] for src in ("rel_attention.hip", "kv_cache.hip", "decode_attention.hip")}
 # -ffp-contract=off: distances are spelled with _rn intrinsics already; this keeps every other
 # f32 expression in the point ops unfused too (parity contract, see oracle/pointnet2_oracle.c).
-LANG_HEADER = os.path.join(CSRC, "lang_core.h")    # of the last three sources only
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on MI355X); the host pass
 # warns that it does not know the feature.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
@@ -54,7 +56,7 @@ def build(force=False, verbose=False):
     for src in sorted(SOURCES, key=lambda f: -cost.get(f, os.path.getsize(os.path.join(CSRC, f)) / 2e4)):
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ, src.replace(".hip", ".o"))
-        if force or _stale(o, [s] + HEADERS + ([LANG_HEADER] if src in SOURCES[-3:] else [])):
+        if force or _stale(o, [s] + HEADERS + HEADERS_OF.get(src, [])):
             jobs.append([hipcc, "-x", "hip", "-c", s, "-o", o] + FLAGS)
 
     def run(cmd):

@@ -1,5 +1,6 @@
 """The build recipe without a compiler: what is compiled again, and when."""
 import os
+import re
 
 import pytest
 
@@ -62,3 +63,29 @@ def test_objects_without_a_record_are_compiled_again(recipe):
     assert recipe()[1]
     os.remove(os.path.join(build.OBJ, "command"))
     assert recipe() == (sorted(build.SOURCES), True)
+
+
+def _included(path, seen):
+    for name in re.findall(r'^#include "([^"]+)"', open(path).read(), re.M):
+        for folder in (os.path.dirname(path), os.path.join(os.path.dirname(path), "..", "..", "include")):
+            at = os.path.normpath(os.path.join(folder, name))
+            if os.path.exists(at) and at not in seen:
+                seen.add(at)
+                _included(at, seen)
+    return seen
+
+
+def test_every_included_header_makes_its_sources_stale(recipe, monkeypatch):
+    """... wherever a source stands in the list."""
+    build = recipe.module
+    monkeypatch.setattr(build, "SOURCES", build.SOURCES[::-1])
+    assert recipe()[1]
+    headers = {src: _included(os.path.join(build.CSRC, src), set()) for src in build.SOURCES}
+    before = {os.path.join(build.OBJ, f): os.path.getmtime(os.path.join(build.OBJ, f)) for f in os.listdir(build.OBJ)}
+    mtime = os.path.getmtime
+    for header in sorted(set().union(*headers.values())):
+        # objects as old as they were, the header newer than they are
+        monkeypatch.setattr(build.os.path, "getmtime", lambda p: before.get(p, 0.0) if not os.path.normpath(p) == header else 1e18)
+        compiled, linked = recipe()
+        monkeypatch.setattr(build.os.path, "getmtime", mtime)
+        assert linked and {s for s in headers if header in headers[s]} <= set(compiled), header
