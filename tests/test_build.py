@@ -89,3 +89,15 @@ def test_every_included_header_makes_its_sources_stale(recipe, monkeypatch):
         compiled, linked = recipe()
         monkeypatch.setattr(build.os.path, "getmtime", mtime)
         assert linked and {s for s in headers if header in headers[s]} <= set(compiled), header
+
+
+def test_the_entry_point_compiles_every_time(monkeypatch):
+    import __graft_entry__
+    from oracle import pointnet2_ref
+    from situation3d_amd import build
+    forced = []
+    monkeypatch.setattr(build, "build", lambda force=False, verbose=False: forced.append(force) or build.LIB)
+    monkeypatch.setattr(pointnet2_ref, "build", lambda force=False: None)
+    monkeypatch.setattr(build.os.path, "exists", lambda p: True)
+    __graft_entry__.build()
+    assert forced == [True]
