@@ -47,9 +47,9 @@ def relative_borders(buckets, max_distance, bidirectional):
         a = found[-1]
         while a ** (n - e) * e ** i < max_distance ** i * e ** (n - e):
             a += 1
+            if a > _lib.REL_MAX_REACH:
+                raise RuntimeError("the last relative position bucket must start at a distance of at most %d" % _lib.REL_MAX_REACH)
         found.append(a)
-    if found[n - 1] > _lib.REL_MAX_REACH:
-        raise RuntimeError("the last relative position bucket must start at a distance of at most %d" % _lib.REL_MAX_REACH)
     return tuple(found[:n])
 
 

@@ -1,4 +1,4 @@
-"""Language-side operators without a GPU: strides of dimensions of one."""
+"""Language-side operators without a GPU: strides of dimensions of one, far distances."""
 import pytest
 import torch
 
@@ -44,3 +44,24 @@ def test_tokens_of_16_mb_are_refused():
     """A dense tensor whose tokens are that long cannot be copied into a shape that the kernels read."""
     q = torch.empty(1, 2, 1 << 17, 64, dtype=torch.float16, device="meta")
     assert not _template(q, q)[1]
+
+
+@pytest.mark.timeout(20)
+@pytest.mark.parametrize("args", [(32, 10 ** 9, True), (32, 10 ** 30, False), (4, 10 ** 12, False), (256, 10 ** 15, True), (128, 1300, False)], ids=str)
+def test_far_distances_are_refused_at_once(args):
+    from situation3d_amd import language
+    with pytest.raises(RuntimeError, match="at most 1024"):
+        language.relative_borders(*args)
+
+
+@pytest.mark.parametrize("args", [(4, 10 ** 6, True), (2, 10 ** 30, False), (3, 1025, False), (64, 1024, False)], ids=str)
+def test_far_distances_that_no_border_stands_at(args):
+    """The last bucket starts before max_distance: there may be but one bucket beyond the single distances, or the last border is near."""
+    from situation3d_amd import language
+    border = language.relative_borders(*args)
+    n = len(border)
+    e, far = n // 2, args[1]
+    assert list(border[:e + 1]) == list(range(e + 1))[:n] and border[-1] <= 1024
+    for i in range(1, n - e):
+        a = border[e + i]
+        assert a ** (n - e) * e ** i >= far ** i * e ** (n - e) > (a - 1) ** (n - e) * e ** i
