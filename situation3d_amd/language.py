@@ -16,7 +16,6 @@ stream of their tensors' device, allocate their outputs and workspaces from torc
 a hipGraph.  GPU tensors only, like the rest of the HIP path.
 """
 import functools
-import math
 
 import torch
 from torch.autograd import forward_ad
@@ -96,6 +95,14 @@ def _launch(name, args, device):
             _lib.call(name, args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def _check_numbers(what, scale, *integers):
+    """An argument struct takes what does not fit modulo 2^32, and a scale beyond float32 (in log2 units) as infinity."""
+    if not all(-1 << 31 <= n < 1 << 31 for n in integers):
+        raise RuntimeError("%s: sizes and positions must be below 2^31" % what)
+    if not abs(scale) < 2.0 ** 127:
+        raise RuntimeError("%s: scale must be finite" % what)
+
+
 def _check_heads(q, k, v, dtypes, what):
     if len(q) != 4 or len(k) != 4 or len(v) != 4:
         raise RuntimeError("%s takes (batch, tokens, heads, head size) tensors" % what)
@@ -158,6 +165,7 @@ def _rel_template(q, qs, k, ks, v, vs, dtypes, table, table_dtype, cfg):
     _check_heads(q, k, v, dtypes, "relative_attention")
     _check_table(table, table_dtype, q[2], dtypes[0], "relative_attention")
     scale, bidirectional, max_distance, causal, offset = cfg
+    _check_numbers("relative_attention", scale, offset, *q, *k)
     rows = 0 if table is None else table[0]
     e = dtypes[0].itemsize
     a = _lib.RelAttentionArgs(dtype=_DTYPES[dtypes[0]], b=q[0], nq=q[1], nk=k[1], h=q[2], hkv=k[2], d=q[3], causal=int(causal),
@@ -287,8 +295,6 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
         raise RuntimeError("relative_attention: prefix_lengths only means something with causal=True")
     cfg = (float(q.shape[-1] ** -0.5 if scale is None else scale), bool(bidirectional), int(max_distance), bool(causal),
            int(query_offset))
-    if not math.isfinite(cfg[0]):
-        raise RuntimeError("relative_attention: scale must be finite")
     if table is not None:
         table = table.contiguous()
     none = (None, None, None)
@@ -374,6 +380,7 @@ class KVCache:
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise RuntimeError("KVCache.append: the cache takes %s" % self.dtype)
         start, counts = _int_array(start, (self.batch,), dev, "start"), _int_array(counts, (self.batch,), dev, "counts")
+        _check_numbers("KVCache.append", 1.0, *shape)
         if shape[1] == 0:
             if start is not None:
                 self._lengths.copy_(start.clamp(0, self.capacity))
@@ -470,8 +477,7 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
 @functools.lru_cache(maxsize=1024)
 def _decode_template(q, qs, dtype, hkv, capacity, quantized, groups, shared_capacity, rows, scale, max_distance, bidirectional):
     """What shapes and types decide of a decode_attention call: its argument struct without addresses, its workspace."""
-    if not math.isfinite(scale):
-        raise RuntimeError("decode_attention: scale must be finite")
+    _check_numbers("decode_attention", scale, *q)
     b, t, h, d = q
     a = _lib.DecodeAttentionArgs(dtype=dtype, b=b, t=t, h=h, hkv=hkv, d=d, capacity=capacity, groups=groups,
                                  shared_capacity=shared_capacity, table_rows=rows, scale=scale,

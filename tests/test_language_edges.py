@@ -1,4 +1,5 @@
-"""Language-side operators without a GPU: strides of dimensions of one, far distances."""
+"""Language-side operators without a GPU: strides of dimensions of one, far distances, numbers
+that an argument struct does not hold."""
 import pytest
 import torch
 
@@ -65,3 +66,24 @@ def test_far_distances_that_no_border_stands_at(args):
     for i in range(1, n - e):
         a = border[e + i]
         assert a ** (n - e) * e ** i >= far ** i * e ** (n - e) > (a - 1) ** (n - e) * e ** i
+
+
+@pytest.mark.parametrize("cfg", [(1e39, True, 128, False, 0), (-2e38, True, 128, False, 0), (float("nan"), True, 128, False, 0),
+                                 (float("inf"), True, 128, False, 0), (1.0, True, 128, True, 1 << 32), (1.0, True, 128, True, 5 - (1 << 33))], ids=str)
+def test_numbers_that_do_not_fit_are_refused(cfg):
+    """2^32 + 5 would be taken as 5."""
+    from situation3d_amd import language
+    q = torch.empty(1, 4, 2, 64)
+    with pytest.raises(RuntimeError):
+        language._rel_template(q.shape, q.stride(), q.shape, q.stride(), q.shape, q.stride(), (q.dtype,) * 3, None, None, cfg)
+    if cfg[4] == 0:
+        with pytest.raises(RuntimeError):
+            language._decode_template((1, 1, 2, 64), (128, 128, 64, 1), 0, 2, 8, False, 0, 0, 0, cfg[0], 128, False)
+
+
+def test_broadcast_tokens_beyond_an_int_are_refused():
+    q, k = torch.empty(1, 4, 2, 64), torch.empty(1, 1, 2, 64).expand(1, (1 << 32) + 5, 2, 64)
+    with pytest.raises(RuntimeError):
+        _template(q, k)
+    with pytest.raises(RuntimeError):
+        _template(q.expand((1 << 32) + 1, 4, 2, 64), k[:, :5].expand((1 << 32) + 1, 5, 2, 64))

@@ -209,3 +209,17 @@ def test_tokens_of_16_mb_are_refused():
     with pytest.raises(RuntimeError, match="16 MB"):
         _lang().relative_attention(q, q, q)
     assert not _lang().relative_attention(q[:, :1], q[:, :1], q[:, :1]).any()      # a single one has no stride
+
+
+def test_numbers_that_do_not_fit_are_refused():
+    lang = _lang()
+    x = torch.zeros(1, 4, 2, 64, device=DEV)
+    cache = lang.KVCache(1, 8, 2, 64, torch.float32, False, DEV)
+    cache.append(x, x)
+    many = x[:, :1].expand(1, (1 << 32) + 3, 2, 64)
+    for bad in (lambda: lang.relative_attention(x, x, x, causal=True, query_offset=1 << 32), lambda: lang.relative_attention(x, x, x, scale=1e39),
+                lambda: lang.relative_attention(x, many, many), lambda: lang.decode_attention(x, cache, scale=-1e39),
+                lambda: lang.decode_attention(x, cache, scale=float("nan")), lambda: cache.append(many, many)):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert cache.lengths.tolist() == [4]
