@@ -293,7 +293,9 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
     _no_tangent("relative_attention", q, k, v, table)
     if prefix_lengths is not None and not causal:
         raise RuntimeError("relative_attention: prefix_lengths only means something with causal=True")
-    cfg = (float(q.shape[-1] ** -0.5 if scale is None else scale), bool(bidirectional), int(max_distance), bool(causal),
+    if q.dim() != 4 or q.shape[3] not in _HEAD_SIZES:
+        raise RuntimeError("relative_attention: q must be (batch, tokens, heads, head size), the head size 64, 96 or 128")
+    cfg = (float(q.shape[3] ** -0.5 if scale is None else scale), bool(bidirectional), int(max_distance), bool(causal),
            int(query_offset))
     if table is not None:
         table = table.contiguous()

@@ -223,3 +223,15 @@ def test_numbers_that_do_not_fit_are_refused():
         with pytest.raises(RuntimeError):
             bad()
     assert cache.lengths.tolist() == [4]
+
+
+@pytest.mark.parametrize("shape", [(), (64,), (2, 3, 4, 0), (2, 3, 4, 80), (2, 3, 4, 64, 1)], ids=str)
+def test_shapes_without_heads_are_refused(shape):
+    x = torch.zeros(shape, device=DEV)
+    with pytest.raises(RuntimeError):
+        _lang().relative_attention(x, x, x)
+    cache = _lang().KVCache(2, 8, 4, 64, torch.float32, False, DEV)
+    with pytest.raises(RuntimeError):
+        cache.append(x, x)
+    with pytest.raises(RuntimeError):
+        _lang().decode_attention(x, cache)
