@@ -33,7 +33,7 @@ struct DecodeParams {
   Side own, shared;
   const int *lengths, *shared_lengths, *counts;
   void *out;
-  float *part;               // pieces: D + 2 floats a row and piece (output, max, sum)
+  float *part;               // pieces: D + 4 floats a row and piece (output, max, sum, two unused)
   long q_b, q_n, q_h;
   int b, t, h, hkv, group, each;       // each: sequences of a shared prefix (0: nothing is shared)
   int own_splits, shared_splits;       // most pieces of a row's own and shared keys (see piece_rows)

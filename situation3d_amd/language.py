@@ -13,7 +13,10 @@ a head is built from, as hand-written HIP kernels (csrc/rel_attention.hip, kv_ca
 Types: float32 (exact-f32 matrix instructions), bfloat16, float16; head sizes 64, 96, 128; grouped key heads (h a multiple of
 hkv).  Statistics, sums and gradients' accumulators are float32; results are rounded once.  All calls run on the current
 stream of their tensors' device, allocate their outputs and workspaces from torch, never synchronise, and may be captured into
-a hipGraph.  GPU tensors only, like the rest of the HIP path.
+a hipGraph (a backward pass like any other of torch's: no eager graph of the same leaves may be alive meanwhile, so make the leaves
+inside the capture).  The same call gives the same bits; how a sum is cut, and in 16 bits how P is rounded (relative_attention),
+follows from the launch's size, so the last bit of a sequence's result may depend on the batch around it.  GPU tensors only, like
+the rest of the HIP path.
 """
 import functools
 
@@ -284,6 +287,9 @@ def relative_attention(q, k, v, table=None, *, scale=None, bidirectional=True, m
       sees may hold anything; those between are finite, also for queries that do not see them.
     A bias of -inf weighs nothing, and neither do float32's and bfloat16's lowest values; a query that sees only such keys
       yields 0 as well.
+    Rounding in 16 bits: P meets V with 16 bits of its own, and once more with what that left, where a backward pass follows or the
+      launch is small; in large launches without one it is rounded once (the result's error 1.4 of one rounding instead of 1.0, so
+      a checkpointed layer's two forward passes differ by that).  There is no dropout of probabilities.
     -> (b, nq, h, d) in q's type."""
     dev = q.device
     if not q.is_cuda:
@@ -424,7 +430,9 @@ def decode_attention(q, cache, shared=None, table=None, *, scale=None, bidirecti
       and before its own tokens -- b / g questions about one scene, read from memory once for all of them.
     table as in relative_attention (keys are never ahead of the query, so bidirectional only says which half of the table
       counts); positions count the shared tokens first.
-    Rows of a cache from its length on may hold anything.
+    Rows of a cache from its length on may hold anything; those before it are finite, also the newest ones for the queries before
+      them.  The queries are those of the last rows held: tokens that append dropped beyond the capacity have none.
+    Cross-attention of one token is decode_attention(q, cache of the encoder's keys), without a table.
     -> (b, t, h, d) in q's type."""
     dev, what = cache.device, "decode_attention"
     if not q.is_cuda or table is not None and not table.is_cuda:

@@ -233,3 +233,20 @@ def test_decoding_errors_as_a_whole(dtype, quantized):
     g = torch.Generator().manual_seed(7)
     _check_decode(g, 3, 2, 16, 4, 128, 2500, (2500, 1, 1300), dtype, quantized)
     _check_decode(g, 24, 1, 16, 4, 64, 100, tuple(range(0, 96, 4)), dtype, quantized, prefix=(1500, 700), shared_capacity=1500, parts=1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=IDS.get)
+@pytest.mark.parametrize("quantized", [False, True], ids=["plain", "e4m3"])
+def test_cross_attention_token_by_token(dtype, quantized):
+    """One answer token over a cache of the encoder's keys: no table, every row held is seen."""
+    lang = _lang()
+    g = torch.Generator().manual_seed(8)
+    lengths = (432, 1, 0, 100)
+    cache = _filled(g, 4, 432, 8, 64, dtype, quantized, lengths)
+    q = torch.randn(4, 1, 8, 64, generator=g).to(dtype).to(DEV)
+    got = lang.decode_attention(q, cache, None, None, scale=1.0)
+    k, v = cache.read()
+    ok = ref.seen(4, 1, 432, key_lengths=_i32(*lengths))
+    want = ref.attention(q, k, v, None, ok, 1.0)
+    ref.check("token", got, want["out"])
+    ref.check("prompt", lang.relative_attention(q, k, v, None, scale=1.0, key_lengths=cache.lengths), want["out"])
