@@ -250,3 +250,20 @@ def test_cross_attention_token_by_token(dtype, quantized):
     want = ref.attention(q, k, v, None, ok, 1.0)
     ref.check("token", got, want["out"])
     ref.check("prompt", lang.relative_attention(q, k, v, None, scale=1.0, key_lengths=cache.lengths), want["out"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_repeated_calls_give_the_same_bits(dtype):
+    """Splits of keys, queries and heads, pieces of shared and own rows: joined in their order, whichever workgroup ends first."""
+    lang = _lang()
+    g = torch.Generator().manual_seed(9)
+    leaves = [x.to(DEV).requires_grad_() for x in acc.inputs(g, 1, 600, 1500, 4, 1, 64, dtype=dtype)]
+    grad = leaves.pop().detach()
+    cache, shared = _filled(g, 6, 2000, 2, 128, dtype, True, (2000, 1, 900, 33, 1999, 0)), _filled(g, 2, 3000, 2, 128, dtype, True, (3000, 700))
+    q, table = torch.randn(6, 2, 16, 128, generator=g).to(dtype).to(DEV), torch.randn(32, 16, generator=g).to(dtype).to(DEV)
+    runs = []
+    for _ in range(4):
+        out = lang.relative_attention(*leaves, causal=True, query_offset=900)
+        runs.append([out.detach(), *torch.autograd.grad(out, leaves, grad), lang.decode_attention(q, cache, shared, table)])
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
