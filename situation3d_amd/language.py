@@ -79,7 +79,7 @@ def _strides(shape, stride):
 
 def _rows(t):
     """`t`, or a dense copy where the kernels cannot read its rows (differentiable)."""
-    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or _readable(t.shape, t.stride(), t.element_size())):
+    if t.data_ptr() % 16 == 0 and (t.is_contiguous() and t.numel() or _readable(t.shape, t.stride(), t.element_size())):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -87,3 +87,12 @@ def test_broadcast_tokens_beyond_an_int_are_refused():
         _template(q, k)
     with pytest.raises(RuntimeError):
         _template(q.expand((1 << 32) + 1, 4, 2, 64), k[:, :5].expand((1 << 32) + 1, 5, 2, 64))
+
+
+def test_no_tokens_of_odd_strides():
+    """Nothing is contiguous whatever its strides; the kernels' view of it is made all the same."""
+    from situation3d_amd import language
+    for t in (torch.empty(2, 0, 2, 65)[..., :64], torch.empty(0, 3, 2, 67)[..., 3:], torch.empty(2, 0, 64, 2).transpose(2, 3)):
+        assert t.is_contiguous() or t.numel() == 0
+        r = language._rows(t)
+        assert r.shape == t.shape and _template(r, torch.empty(r.shape[0], 5, 2, 64))[1]

@@ -235,3 +235,11 @@ def test_shapes_without_heads_are_refused(shape):
         cache.append(x, x)
     with pytest.raises(RuntimeError):
         _lang().decode_attention(x, cache)
+
+
+def test_no_tokens_of_odd_strides():
+    x, none = torch.randn(2, 3, 2, 64, device=DEV), torch.empty(2, 0, 2, 65, device=DEV)[..., :64]
+    assert _lang().relative_attention(none, x, x).shape == (2, 0, 2, 64)
+    x.requires_grad_()
+    out = _lang().relative_attention(x, none, none)
+    assert not out.any() and not torch.autograd.grad(out.sum(), x)[0].any()
