@@ -388,7 +388,8 @@ class KVCache:
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise RuntimeError("KVCache.append: the cache takes %s" % self.dtype)
         start, counts = _int_array(start, (self.batch,), dev, "start"), _int_array(counts, (self.batch,), dev, "counts")
-        _check_numbers("KVCache.append", 1.0, *shape)
+        if shape[1] >= 1 << 31:                          # (broadcast: the struct would take them modulo 2^32)
+            raise RuntimeError("KVCache.append: %d tokens" % shape[1])
         if shape[1] == 0:
             if start is not None:
                 self._lengths.copy_(start.clamp(0, self.capacity))
